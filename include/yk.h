@@ -259,6 +259,117 @@ yk_status yk_forward_step_split(yk_model* m, yk_kv_pool* pool, yk_kv_pool* wpool
 /* Copies logits rows [row0, row0+rows) of the last forward step to host (tests). */
 yk_status yk_logits_copy_to_host(yk_model* m, int32_t row0, int32_t rows, float* host);
 
+/* ---- operators on a paged KV cache in device memory.  No counterpart in the
+ * reference (its cache is fp32, written by PagedKVCache.appendFromFull,
+ * S/PagedKVCache.swift:24-62, and read by batched_paged_attention_kernel,
+ * S/gemm.metal:629-737).  Both calls take device pointers of `device` and a
+ * cudaStream_t, allocate nothing, never wait for the device, may be captured
+ * into a CUDA graph and are complete when the stream is.  Arguments are checked
+ * before anything is launched (YK_ERR_ARG, YK_ERR_UNSUPPORTED); a CUDA error
+ * left pending by earlier work on the calling thread is returned as YK_ERR_CUDA
+ * and nothing is launched.  What only the device can see (a slot or block
+ * outside the pool, lengths that do not fit) is skipped there and sets
+ * YK_DEV_ERR_BOUNDS (1) in *err; err may be null. ----------------------------- */
+#define YK_KV_F32  0 /* cells fp32                                               */
+#define YK_KV_BF16 1 /* cells bf16                                               */
+#define YK_KV_E4M3 2 /* cells of 8 bits (e4m3), one scale byte per block and head */
+/* A pool's memory: cells [block][layer][K|V][kv head][16][head_dim].  YK_KV_E4M3:
+ * scales [block][layer][K|V][kv head], one byte each; a cell stands for
+ * code * 2^(byte - 127), the byte in 67..187 (a byte outside is read as the
+ * nearest of them).  data is 16-byte aligned; head_dim 64, 128 or 256. */
+typedef struct yk_kv_pages {
+    void*    data;
+    uint8_t* scales;     /* YK_KV_E4M3 only, else null                           */
+    int32_t  kind;       /* YK_KV_*                                              */
+    int32_t  num_blocks;
+    int32_t  n_layers;   /* layers per block                                     */
+    int32_t  n_kv_heads;
+    int32_t  head_dim;
+} yk_kv_pages;
+
+/* Between the QKV product and attention, in one pass over the projections:
+ * row t of qkv holds n_heads query heads, then n_kv_heads key heads, then
+ * n_kv_heads value heads, head_dim values each.
+ *   norm      queries and keys, per head: x / sqrt(mean(x^2) + eps) * gain
+ *             (q_gain / k_gain [head_dim] fp32; null: no norm)
+ *   rotation  of the pairs (2i, 2i+1) of queries and keys by rope[t][i] =
+ *             (cos, sin), fp32 (S/gemm.metal:674-682); null: none
+ *   store     queries to q_out, keys and values to cache slot slots[t] =
+ *             block * 16 + offset of layer `layer`.
+ * A negative slot marks a row of padding: nothing of it is read or written.  No
+ * slot may appear twice, and the rows of one block must follow one another (rows
+ * of padding may lie between them).
+ * YK_KV_E4M3: the exponent of a block's K (or V) of one head is the smallest in
+ * -60..60 whose 448 * 2^e covers the finite new values; when older tokens stay
+ * in the block (cells below its last new one that are not new) it never falls
+ * below the one it had, and if it rises their cells are rounded again to the new
+ * one.  Cells past the last new one are left as they are.  Values round to
+ * nearest even; larger ones, infinities included, become +-448 * 2^e, NaN stays
+ * NaN.
+ * src_dtype / q_dtype: F32 -> F32, F32 -> BF16 or BF16 -> BF16; cells fp32 or
+ * bf16 must have q_dtype's type.  qkv and q_out are 16-byte aligned, strides
+ * (elements between tokens) multiples of 16 bytes. */
+typedef struct yk_kv_append_args {
+    yk_kv_pages    pages;
+    int32_t        layer;
+    int32_t        T;          /* rows of qkv, q_out, slots and rope; 0: nothing is done */
+    int32_t        n_heads;
+    int32_t        src_dtype;  /* YK_DTYPE_* of qkv                                 */
+    int32_t        q_dtype;    /* YK_DTYPE_* of q_out                               */
+    float          eps;
+    const void*    qkv;
+    int64_t        qkv_stride;
+    void*          q_out;
+    int64_t        q_stride;
+    const int32_t* slots;
+    const float*   rope;       /* [T][head_dim / 2][2]                              */
+    const float*   q_gain;
+    const float*   k_gain;
+    uint32_t*      err;
+} yk_kv_append_args;
+yk_status yk_kv_append(int32_t device, void* stream, const yk_kv_append_args* args);
+
+/* Causal attention of a ragged batch over an e4m3 paged cache (one layer): token
+ * i of sequence b sits at position p = context_lens[b] - n_b + i, n_b =
+ * q_starts[b+1] - q_starts[b], and attends to the cached keys j <= p (window >
+ * 0: and p - j < window) through its row of block_tables; its own key must be in
+ * the cache.  Query head h reads KV head h / (n_heads / n_kv_heads).  Scores are
+ * scaled by `scale` (0: head_dim^-1/2) and soft-capped, cap * tanh(s / cap),
+ * when cap > 0.  A token without a visible key (a position below 0) gets zeros;
+ * rows of out from q_starts[B] on are left as they were, and cells that a query
+ * does not attend to never reach its result, whatever they hold.
+ * max_new: no sequence brings more new tokens than this (0: unknown); a wrong
+ * value costs time, not correctness.  q, out: [T][n_heads][head_dim] with the
+ * given strides (elements between tokens, multiples of 16 bytes; bases 16-byte
+ * aligned), both F32 or both BF16.
+ * workspace: yk_attention_e4m3_workspace bytes, 16-byte aligned, zeroed once by
+ * the caller before its first use; every call leaves it ready for the next.
+ * Calls that overlap on the GPU need a workspace each. */
+typedef struct yk_attention_e4m3_args {
+    yk_kv_pages    pages;
+    int32_t        layer;
+    int32_t        T;            /* rows of q and out; 0: nothing is done            */
+    int32_t        B;
+    int32_t        n_heads;
+    int32_t        dtype;        /* YK_DTYPE_* of q and out                          */
+    int32_t        max_blocks;   /* columns of block_tables                          */
+    int32_t        max_new;
+    int32_t        window;
+    float          scale, cap;
+    const void*    q;
+    int64_t        q_stride;
+    void*          out;
+    int64_t        out_stride;
+    const int32_t* q_starts;     /* [B + 1], from 0, not falling, at most T          */
+    const int32_t* context_lens; /* [B]                                             */
+    const int32_t* block_tables; /* [B][max_blocks]                                 */
+    void*          workspace;
+    uint64_t       workspace_bytes;
+    uint32_t*      err;
+} yk_attention_e4m3_args;
+yk_status yk_attention_e4m3(int32_t device, void* stream, const yk_attention_e4m3_args* args);
+yk_status yk_attention_e4m3_workspace(int32_t device, int32_t head_dim, uint64_t* bytes);
+
 /* ---- sampler.  Replaces SpeculativeSampler (S/SpeculativeSampler.swift) and
  * the Scheduler's draft sampling (S/Scheduler.swift:171-189).  Uniform draws
  * are Philox4x32-10 keyed by seed, counter (step, seq_id, position, slot) with

@@ -22,6 +22,7 @@ BLOCK_SIZE = 16
 (T_EMBED, T_WQ, T_WK, T_WV, T_WO, T_WGATE, T_WUP, T_WDOWN, T_NORM1, T_NORM2, T_FINAL_NORM,
  T_LM_HEAD) = range(12)
 LAYOUT_OUT_IN, LAYOUT_IN_OUT = 0, 1
+KV_F32, KV_BF16, KV_E4M3 = 0, 1, 2
 
 
 class ModelConfig(C.Structure):
@@ -46,6 +47,30 @@ def make_config(**kw) -> ModelConfig:
     for k, v in defaults.items():
         setattr(c, k, v)
     return c
+
+
+class KVPages(C.Structure):
+    """yk_kv_pages (include/yk.h): a paged KV pool's device memory."""
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("kind", C.c_int32), ("num_blocks", C.c_int32),
+                ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class KVAppendArgs(C.Structure):
+    """yk_kv_append_args (include/yk.h)."""
+    _fields_ = [("pages", KVPages), ("layer", C.c_int32), ("T", C.c_int32), ("n_heads", C.c_int32),
+                ("src_dtype", C.c_int32), ("q_dtype", C.c_int32), ("eps", C.c_float), ("qkv", C.c_void_p),
+                ("qkv_stride", C.c_int64), ("q_out", C.c_void_p), ("q_stride", C.c_int64), ("slots", C.c_void_p),
+                ("rope", C.c_void_p), ("q_gain", C.c_void_p), ("k_gain", C.c_void_p), ("err", C.c_void_p)]
+
+
+class AttentionE4M3Args(C.Structure):
+    """yk_attention_e4m3_args (include/yk.h)."""
+    _fields_ = [("pages", KVPages), ("layer", C.c_int32), ("T", C.c_int32), ("B", C.c_int32), ("n_heads", C.c_int32),
+                ("dtype", C.c_int32), ("max_blocks", C.c_int32), ("max_new", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float), ("cap", C.c_float), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("q_starts", C.c_void_p),
+                ("context_lens", C.c_void_p), ("block_tables", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64), ("err", C.c_void_p)]
 
 
 class YKError(RuntimeError):
@@ -120,6 +145,9 @@ _PROTOS = {
     "yk_tp_allgather_u32": (C.c_int32, [_P, _U32P, C.c_int32, _U32P]),
     "yk_spec_verify_logits_noalloc": (C.c_int32, [C.c_int32, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                                   C.c_float, C.c_uint64, C.c_uint32, _P, _P]),
+    "yk_kv_append": (C.c_int32, [C.c_int32, _P, C.POINTER(KVAppendArgs)]),
+    "yk_attention_e4m3": (C.c_int32, [C.c_int32, _P, C.POINTER(AttentionE4M3Args)]),
+    "yk_attention_e4m3_workspace": (C.c_int32, [C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
     # include/yk_testing.h
     "ykt_gemm_bf16": (C.c_int32, [_P, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16), C.c_int32, C.c_int32,
                                   C.c_int32, C.c_int32, _F32P]),
@@ -285,6 +313,120 @@ def tp_unique_id() -> bytes:
     buf = (C.c_uint8 * 128)()
     check(lib().yk_tp_unique_id(buf))
     return bytes(buf)
+
+
+# ---------------------------------------------------------------------------
+# Operators on a paged KV cache held in torch CUDA tensors (include/yk.h).
+# Tensors are used in place, on the device they share and on its current torch
+# stream (or `stream`, a cudaStream_t); nothing is copied, cast or kept.
+# ---------------------------------------------------------------------------
+def _code(t, name: str) -> int:
+    import torch
+
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    raise ValueError(f"{name}: float32 or bfloat16, not {t.dtype}")
+
+
+def _address(t, name: str, device: int, size: int, numel: int | None = None, whole: bool = False):
+    """data_ptr of a contiguous tensor on `device` with elements of `size` bytes (None: null);
+    whole: of integers."""
+    if t is None:
+        return None
+    if whole and t.dtype.is_floating_point:
+        raise ValueError(f"{name} must hold 32-bit integers")
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{name} is not on cuda:{device}")
+    if t.element_size() != size or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with {size}-byte elements")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must have {numel} elements, not {t.numel()}")
+    return t.data_ptr()
+
+
+def kv_pages(pool, scales, device: int) -> KVPages:
+    """pool [blocks, layers, 2, kv heads, 16, head_dim]: 1-byte elements with scales
+    [blocks, layers, 2, kv heads] (1-byte elements), or fp32 / bf16 and scales None."""
+    if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[4] != BLOCK_SIZE:
+        raise ValueError("pool must be [blocks, layers, 2, kv heads, 16, head_dim]")
+    n, layers, _, g, _, dh = pool.shape
+    size = pool.element_size()
+    if size == 1:
+        if scales is None:
+            raise ValueError("a pool of 8-bit cells needs scales")
+        kind = KV_E4M3
+    else:
+        kind = KV_F32 if _code(pool, "pool") == DTYPE_F32 else KV_BF16
+    return KVPages(_address(pool, "pool", device, size), _address(scales, "scales", device, 1, n * layers * 2 * g),
+                   kind, n, layers, g, dh)
+
+
+def _rows(t, name: str, device: int, tokens: int, heads: int, dh: int):
+    """(address, elements between tokens) of [tokens, heads, head_dim] (or [tokens, heads * head_dim])."""
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{name} is not on cuda:{device}")
+    s = t.stride()
+    tail = s[1:] == (dh, 1) and t.shape[1:] == (heads, dh) if t.dim() == 3 else t.dim() == 2 and \
+        s[1] == 1 and t.shape[1] == heads * dh
+    if t.shape[0] != tokens or not tail:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {dh}] with contiguous rows")
+    return t.data_ptr(), (s[0] if tokens > 1 else heads * dh)
+
+
+def _stream(device: int, stream):
+    if stream is None:
+        import torch
+
+        return torch.cuda.current_stream(device).cuda_stream
+    return stream
+
+
+def kv_append(pool, scales, layer: int, qkv, q_out, slots, rope, q_gain, k_gain, eps: float, err, heads: int,
+              stream=None) -> None:
+    """yk_kv_append: norms and rotation of the queries and keys of qkv [T, (heads + 2 kv heads) * head_dim],
+    queries to q_out [T, heads, head_dim], keys and values to cache slots [T] (int32) of `layer`.
+    rope [T, head_dim / 2, 2], q_gain / k_gain [head_dim]: fp32 or None; err: int32 [1] or None."""
+    dev = qkv.get_device()
+    pages = kv_pages(pool, scales, dev)
+    g, dh, n = pages.n_kv_heads, pages.head_dim, slots.numel()
+    a = KVAppendArgs(pages, layer, n, heads, _code(qkv, "qkv"), _code(q_out, "q_out"), eps,
+                     *_rows(qkv, "qkv", dev, n, heads + 2 * g, dh), *_rows(q_out, "q_out", dev, n, heads, dh),
+                     _address(slots, "slots", dev, 4, whole=True), _address(rope, "rope", dev, 4, n * dh),
+                     _address(q_gain, "q_gain", dev, 4, dh), _address(k_gain, "k_gain", dev, 4, dh),
+                     _address(err, "err", dev, 4))
+    check(lib().yk_kv_append(dev, _stream(dev, stream), C.byref(a)))
+
+
+def attention_e4m3(q, out, pool, scales, layer: int, q_starts, context_lens, block_tables, workspace, err, *,
+                   max_new: int = 0, window: int = 0, scale: float = 0.0, cap: float = 0.0, stream=None) -> None:
+    """yk_attention_e4m3: causal attention of q [T, heads, head_dim] over the e4m3 cache, into out.
+    q_starts [B + 1], context_lens [B], block_tables [B, max_blocks]: int32; workspace: bytes (at least
+    attention_e4m3_workspace(...)), zeroed once by the caller; err: int32 [1] or None."""
+    dev = q.get_device()
+    pages = kv_pages(pool, scales, dev)
+    if q.dim() != 3 or block_tables.dim() != 2:
+        raise ValueError("q must be [T, heads, head_dim], block_tables [B, max_blocks]")
+    n, heads, dh = q.shape
+    B, width = block_tables.shape
+    if dh != pages.head_dim or out.dtype != q.dtype:
+        raise ValueError("q, out and the pool disagree on head_dim or dtype")
+    a = AttentionE4M3Args(pages, layer, n, B, heads, _code(q, "q"), width, max_new, window, scale, cap,
+                          *_rows(q, "q", dev, n, heads, dh), *_rows(out, "out", dev, n, heads, dh),
+                          _address(q_starts, "q_starts", dev, 4, B + 1, True),
+                          _address(context_lens, "context_lens", dev, 4, B, True),
+                          _address(block_tables, "block_tables", dev, 4, whole=True),
+                          _address(workspace, "workspace", dev, workspace.element_size()),
+                          workspace.numel() * workspace.element_size(), _address(err, "err", dev, 4))
+    check(lib().yk_attention_e4m3(dev, _stream(dev, stream), C.byref(a)))
+
+
+def attention_e4m3_workspace(head_dim: int, device: int = 0) -> int:
+    """Bytes of workspace yk_attention_e4m3 needs on `device`."""
+    n = C.c_uint64()
+    check(lib().yk_attention_e4m3_workspace(device, head_dim, C.byref(n)))
+    return n.value
 
 
 # ---------------------------------------------------------------------------
