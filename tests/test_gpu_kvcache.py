@@ -68,17 +68,17 @@ class Attention:
 
     def check(self, err=0, **kw):
         ref_kw = {k: v for k, v in kw.items() if k in ("window", "scale", "cap")}
-        want, weight, spread = ref.attention(self.q, self.pool, self.scales, self.layer, self.starts, self.ctx,
+        want, weight, spread, floor = ref.attention(self.q, self.pool, self.scales, self.layer, self.starts, self.ctx,
                                              self.tables, **ref_kw)
         self.call(**kw)
         torch.cuda.synchronize()
-        self.compare(want, weight, spread, err)
+        self.compare(want, weight, spread, floor, err)
 
-    def compare(self, want, weight, spread, err=0):
+    def compare(self, want, weight, spread, floor, err=0):
         got = self.out.double().cpu()
         n = self.starts[-1]
         assert (got[n:] == 7.0).all(), "rows behind the last sequence were written"
-        bound = ref.attention_bound(want[:n], weight[:n], spread[:n], want.shape[-1], self.out.dtype)
+        bound = ref.attention_bound(want[:n], weight[:n], spread[:n], floor[:n], want.shape[-1], self.out.dtype)
         off = (got[:n] - want[:n]).abs()
         assert not torch.isnan(got[:n]).any()
         worst = float((off / bound).max()) if n else 0.0
@@ -181,7 +181,7 @@ def test_attention_nan_in_masked_cells(dtype, dh):
 def test_attention_nan_cell_reaches_those_who_see_it(dtype, dh, which):
     """A NaN in the K or V of one new token: earlier tokens are untouched, later ones are NaN."""
     a = Attention(16, 4, 2, dh, [(8, 60), (1, 20)], dtype)
-    want, weight, spread = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
+    want, weight, spread, floor = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
     j = 60 - 3  # the sixth new token's cell
     a.pool[a.tables[0, j // 16], 1, which, 0, j % 16, 5] = 0xFF
     a.call()
@@ -193,7 +193,7 @@ def test_attention_nan_cell_reaches_those_who_see_it(dtype, dh, which):
     else:
         clean[5:8, :2, 5] = False
     assert torch.isnan(got[~clean]).all()
-    bound = ref.attention_bound(want, weight, spread, dh, a.out.dtype)
+    bound = ref.attention_bound(want, weight, spread, floor, dh, a.out.dtype)
     assert ((got - want).abs()[clean] <= bound[clean]).all()
 
 
@@ -600,8 +600,8 @@ def test_append_then_attend_over_a_growing_cache(dtype):
             abi.kv_append(pool, scales, layer, qkv, q, slots, rope, gain, gain, 1e-6, err, H)
             abi.attention_e4m3(q, out, pool, scales, layer, i32(starts), i32(ctx), i32(tables), ws, err, max_new=max(new))
             torch.cuda.synchronize()
-            want, weight, spread = ref.attention(q, pool, scales, layer, starts, ctx, tables)
-            bound = ref.attention_bound(want, weight, spread, dh, q.dtype)
+            want, weight, spread, floor = ref.attention(q, pool, scales, layer, starts, ctx, tables)
+            bound = ref.attention_bound(want, weight, spread, floor, dh, q.dtype)
             assert ((out.double().cpu() - want).abs() <= bound).all()
             # and the cache holds what was appended, to half a step of its blocks' largest
             x = ref.rotated(ref.normed(qkv.double().cpu().view(-1, H + 2 * G, dh)[:, H:H + G], gain.cpu(), 1e-6), rope.cpu())
