@@ -23,6 +23,8 @@ struct Attn8Params {
     long long block_scales, layer_scale;
     int T, B, H, G, layer, max_blocks, num_blocks;
     int lg;             // log2 of the row groups
+    uint32_t rep_magic;  // ceil(2^32 / (H / G)), 0 where that is 1
+    unsigned long long grid_magic;  // the same for the grid size and 64-bit x
     int window;
     float scale_log2, cap, cap_log2, inv_cap_log2;  // _log2: times log2(e)
 };
@@ -70,7 +72,10 @@ __host__ __device__ constexpr int a8_max_nt() {
 }
 
 struct Seg {
-    int b, qt, g;
+    int b, g;
+    int tok, rem;    // first row of the tile: token tok of the batch, query head rem of the group
+    int rows;
+    int pos;         // position of that token
     int page, pend;  // first page of this CTA's part; pages of the span's keys end here
     int v, n;        // its place and length (pages) in the CTA's range
     int c0, c1;      // first and last CTA of the span
@@ -85,11 +90,15 @@ struct A8Cfg {
     static constexpr int BOXES = DH / ROWB;
     static constexpr int PAGE = 32 * DH;
     static constexpr int DEPTH = A8_RING / 4 / PAGE;  // pages of a warp's share of the ring
-    static constexpr bool QREG = TERMS * NT * KS * 2 <= 48;  // queries in registers, else shared memory
-    static constexpr int QBYTES = QREG ? 0 : 2 * TERMS * NT * KS * 256;  // (two row groups)
-    static constexpr int DUMP = 2 * NT * MT * 512;           // two warps' accumulators
+    static constexpr bool QREG = TERMS * NT * KS * 2 <= 48;  // queries in registers through the page loop
+    static constexpr int ROWS = 8 * NT;                      // of a warp
+    static constexpr int QBYTES = 2 * TERMS * NT * KS * 256;  // fragments of two row groups
+    static constexpr int LDO = DH + 4;                       // floats of an accumulator row
+    static constexpr int DUMP = 2 * ROWS * LDO * 4;          // accumulators of two warps
     static constexpr int SHARED = QBYTES > DUMP ? QBYTES : DUMP;  // used in turn
-    static constexpr size_t SMEM = 1024 + A8_RING + SHARED + 4 * NT * 8 * 8 + A8_SEGS * sizeof(Seg) + 2 * 4 * DEPTH * 8 + 256;
+    static constexpr int NANS = 2 * ROWS * (DH / 32) * 4;    // bit per (row, dim)
+    static constexpr size_t SMEM = 1024 + A8_RING + SHARED + NANS + 4 * ROWS * 8 + 2 * ROWS * 8 + 2 * ROWS * 4 +
+                                   2 * 4 * DEPTH * 8 + A8_SEGS * sizeof(Seg) + 128;
 };
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
@@ -131,59 +140,82 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
+// tanh to a few 2^-24 of its value: 1 - 2 / (1 + e^2z) away from 0, the odd
+// series z - z^3/3 + 2z^5/15 - 17z^7/315 near it.
+__device__ __forceinline__ float tanh_cap(float z) {
+    const float e = 1.f - __fdividef(2.f, 1.f + ex2(fminf(z * 2.8853900817779268f, 126.f)));
+    const float q = z * z, t = fmaf(fmaf(fmaf(-17.f / 315.f, q, 2.f / 15.f), q, -1.f / 3.f), q, 1.f) * z;
+    return fabsf(z) < 0.25f ? t : e;
+}
+
+// x / (H / G), x below 64 + H / G (exact: x * (H / G) < 2^32).
+__device__ __forceinline__ int div_rep(const Attn8Params& p, int x) {
+    return p.rep_magic ? (int)__umulhi((unsigned)x, p.rep_magic) : x;
+}
+
 // A span's pages: [page, pend), at least one (page == pend: a tile without keys).
 struct Span {
-    int rows, page, pend;
+    int rows, page, pend, tok, rem;  // tok: of the sequence
     __device__ __forceinline__ int units() const { return max(1, pend - page); }
 };
 __device__ __forceinline__ Span span_of(const Attn8Params& p, int n, int ctx, int qt, int R, int rep) {
-    const int lo = (int)((long long)qt * R), hi = (int)min((long long)n * rep, (long long)lo + R);
-    const int first = ctx - n + lo / rep, last = ctx - n + (hi - 1) / rep;
+    const long long lo = (long long)qt * R;
     Span s;
-    s.rows = hi - lo;
+    s.rows = (int)min((long long)n * rep - lo, (long long)R);
+    s.tok = (int)((unsigned)lo / (unsigned)rep);
+    s.rem = (int)lo - s.tok * rep;
+    const int first = ctx - n + s.tok;
+    const int last = first + div_rep(p, s.rem + s.rows - 1);
     s.pend = (int)((min(max((long long)last + 1, 0LL), (long long)p.max_blocks * 16) + 15) >> 4);
     s.page = p.window > 0 ? min(max(0, first - p.window + 1) >> 4, s.pend) : 0;
     return s;
 }
 
-// New tokens of sequence b; 0 (and the error word) where q_starts does not fit.
+// New tokens of sequence b; 0 where q_starts does not fit.
 __device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& start) {
     start = p.q_starts[b];
     const int end = p.q_starts[b + 1];
-    const bool ok = start >= 0 && end >= start && end <= p.T && (b > 0 || start == 0);
-    if (!ok) raise_err(p.err, YK_DEV_ERR_BOUNDS);
-    return ok ? end - start : 0;
+    return start >= 0 && end >= start && end <= p.T && (b > 0 || start == 0) ? end - start : -1;
 }
 
 template <typename AT, int DH, int NT>
 __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
     attn8_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
     using C = A8Cfg<AT, DH, NT>;
-    constexpr int TERMS = C::TERMS, KS = C::KS, MT = C::MT, NH = DH / 64;
+    constexpr int TERMS = C::TERMS, KS = C::KS, MT = C::MT, NH = DH / 64, D4 = DH / 4;
+    constexpr float LOWEST = -3.402823466e38f, LARGEST = 3.402823466e38f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* const shared = ring + A8_RING;  // queries during a span, accumulators at its end
-    float2* const s_ml = reinterpret_cast<float2*>(shared + C::SHARED);  // [4 warps][8 * NT] (m, l)
-    Seg* const segs = reinterpret_cast<Seg*>(s_ml + 4 * 8 * NT);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(segs + A8_SEGS);
-    long long* const s_scan = reinterpret_cast<long long*>(bars + 2 * 4 * C::DEPTH);  // [4] + [4]
-    int* const s_flag = reinterpret_cast<int*>(s_scan + 8);
+    uint8_t* const shared = ring + A8_RING;  // queries at the start of a span, accumulators at its end
+    float* const s_o = reinterpret_cast<float*>(shared);                     // [2][ROWS][LDO]
+    uint32_t* const s_nan = reinterpret_cast<uint32_t*>(shared + C::SHARED);  // [2 * ROWS][DH / 32]
+    float2* const s_ml = reinterpret_cast<float2*>(s_nan + C::NANS / 4);      // [4 warps][ROWS] (m, l)
+    float2* const s_row = s_ml + 4 * C::ROWS;                                 // [2 * ROWS] joined (m, l)
+    float* const s_rf = reinterpret_cast<float*>(s_row + 2 * C::ROWS);        // [2 * ROWS] score factor
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(s_rf + 2 * C::ROWS);
+    Seg* const segs = reinterpret_cast<Seg*>(bars + 2 * 4 * C::DEPTH);
+    long long* const s_units = reinterpret_cast<long long*>(segs + A8_SEGS);  // [4]
+    int* const s_spans = reinterpret_cast<int*>(s_units + 4);                 // [4]
+    int* const s_flag = s_spans + 4;  // [0] first span, [1] last span, [2] last arriver, [3] NaN cells seen
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r = lane >> 2, c = lane & 3;
     const int RG = 1 << p.lg, nparts = 4 >> p.lg;
     const int part = warp >> p.lg, rg = warp & (RG - 1);
     const int depth = C::DEPTH << p.lg;
-    const int R = 8 * NT * RG, rep = p.H / p.G;
+    const int R = C::ROWS * RG, rep = p.H / p.G;
+    const int my0 = rg * C::ROWS;  // this warp's first row of a tile
     const uint32_t my_ring = smem_u32(ring) + (uint32_t)(part * depth * C::PAGE);
     const uint32_t full = smem_u32(bars + part * depth), empty = smem_u32(bars + 4 * C::DEPTH + part * depth);
 
+    for (int i = threadIdx.x; i < 4 * C::DEPTH; i += A8_THREADS) {
+        mbar_init(smem_u32(bars + i), 1);
+        mbar_init(smem_u32(bars + 4 * C::DEPTH + i), (uint32_t)RG);
+    }
+    for (int i = threadIdx.x; i < C::NANS / 4; i += A8_THREADS) s_nan[i] = 0;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 * C::DEPTH; ++i) {
-            mbar_init(smem_u32(bars + i), 1);
-            mbar_init(smem_u32(bars + 4 * C::DEPTH + i), (uint32_t)RG);
-        }
         mbar_fence_init();
+        s_flag[3] = 0;
     }
     pdl_trigger();
     pdl_wait();
@@ -191,70 +223,47 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
     // ---- this CTA's range of pages: [lo, hi) of the spans laid end to end
     const int per_thread = (p.B + A8_THREADS - 1) / A8_THREADS;
     const int b_lo = min(p.B, (int)threadIdx.x * per_thread), b_hi = min(p.B, b_lo + per_thread);
-    long long mine = 0;
+    long long units = 0;
+    int spans = 0;
     for (int b = b_lo; b < b_hi; ++b) {
         int start;
         const int n = new_tokens(p, b, start), ctx = p.ctx[b];
-        if (n > 0 && ctx > p.max_blocks * 16LL) raise_err(p.err, YK_DEV_ERR_BOUNDS);
-        const int tiles = (int)(((long long)n * rep + R - 1) / R);
-        for (int qt = 0; qt < tiles; ++qt) mine += (long long)span_of(p, n, ctx, qt, R, rep).units() * p.G;
+        if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
+        for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+            units += (long long)span_of(p, n, ctx, qt, R, rep).units() * p.G;
+            spans += p.G;
+        }
     }
-    long long before = mine;  // inclusive, then exclusive prefix over the threads
+    long long at0 = units;  // exclusive prefixes over the threads
+    int ord0 = spans;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
+        const long long x = __shfl_up_sync(0xffffffffu, at0, o);
+        const int y = __shfl_up_sync(0xffffffffu, ord0, o);
+        if (lane >= o) {
+            at0 += x;
+            ord0 += y;
+        }
     }
-    if (lane == 31) s_scan[warp] = before;
+    if (lane == 31) {
+        s_units[warp] = at0;
+        s_spans[warp] = ord0;
+    }
     __syncthreads();
     long long total = 0;
-    before -= mine;
+    at0 -= units;
+    ord0 -= spans;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        if (w < warp) before += s_scan[w];
-        total += s_scan[w];
+        if (w < warp) {
+            at0 += s_units[w];
+            ord0 += s_spans[w];
+        }
+        total += s_units[w];
     }
-    const long long per = max((long long)A8_MIN_UNITS, (total + gridDim.x - 1) / gridDim.x);
+    const long long per = max((long long)A8_MIN_UNITS, (long long)__umul64hi((unsigned long long)(total + gridDim.x - 1), p.grid_magic));
     const long long lo = (long long)blockIdx.x * per, hi = min(total, lo + per);
     if (lo >= hi) return;
-
-    // the spans of [lo, hi), numbered in order, A8_SEGS of them at a time
-    const auto each_span = [&](auto&& f) {
-        if (before >= hi || before + mine <= lo) return;
-        long long at = before;
-        for (int b = b_lo; b < b_hi; ++b) {
-            const int s0 = p.q_starts[b], s1 = p.q_starts[b + 1];
-            const int n = s0 >= 0 && s1 >= s0 && s1 <= p.T && (b > 0 || s0 == 0) ? s1 - s0 : 0, ctx = p.ctx[b];
-            const int tiles = (int)(((long long)n * rep + R - 1) / R);
-            for (int qt = 0; qt < tiles; ++qt) {
-                const Span s = span_of(p, n, ctx, qt, R, rep);
-                const long long u = s.units(), end = at + u * p.G;
-                if (end > lo && at < hi) {
-                    const int g0 = (int)(at >= lo ? 0 : (lo - at) / u);
-                    const int g1 = (int)(end <= hi ? p.G : (hi - at + u - 1) / u);
-                    for (int g = g0; g < g1; ++g) f(b, qt, g, s, at + g * u, u);
-                }
-                at = end;
-            }
-        }
-    };
-    int count = 0;
-    each_span([&](int, int, int, const Span&, long long, long long) { ++count; });
-    int first = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, first, o);
-        if (lane >= o) first += x;
-    }
-    if (lane == 31) s_scan[4 + warp] = first;
-    __syncthreads();
-    int nspans = 0;
-    first -= count;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < warp) first += (int)s_scan[4 + w];
-        nspans += (int)s_scan[4 + w];
-    }
 
     // per-thread places in a page: K rows sigma(r), sigma(r) + 8; V rows c, c + 4, c + 8, c + 12
     const int sigma = (r & 1) * 4 + (r >> 1);
@@ -279,30 +288,67 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
 
     bool dead = false;  // a bounded wait ran out: nothing more is loaded or computed
     int done = 0;       // pages this part has been through (ring slots and phases follow from it)
-    for (int seg0 = 0; seg0 < nspans; seg0 += A8_SEGS) {
-        __syncthreads();
-        {
-            int i = first - seg0;
-            each_span([&](int b, int qt, int g, const Span& s, long long at, long long u) {
-                if (i >= 0 && i < A8_SEGS) {
-                    const long long from = max(at, lo), to = min(at + u, hi);
-                    segs[i] = Seg{b, qt, g, s.page + (int)(from - at), s.pend, (int)(from - lo), (int)(to - from),
-                                  (int)(at / per), (int)((at + u - 1) / per)};
+    int first = 0, nspans = 0;
+    // the spans of [lo, hi), A8_SEGS of them at a time; the first turn only counts them
+    for (int seg0 = -A8_SEGS; seg0 < nspans; seg0 += A8_SEGS) {
+        if (at0 < hi && at0 + units > lo) {
+            long long at = at0;
+            int ord = ord0;
+            for (int b = b_lo; b < b_hi; ++b) {
+                int start;
+                const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+                for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+                    const Span s = span_of(p, n, ctx, qt, R, rep);
+                    const int u = s.units();
+                    const long long end = at + (long long)u * p.G;
+                    if (end > lo && at < hi) {
+                        // heads [g0, g1) overlap (a tile's heads hold less than 2^31 pages)
+                        const int g0 = at >= lo ? 0 : (int)((unsigned)(lo - at) / (unsigned)u);
+                        const int g1 = end <= hi ? p.G : (int)((unsigned)(hi - at + u - 1) / (unsigned)u);
+                        if (seg0 < 0) {
+                            if (at <= lo) s_flag[0] = ord + g0;
+                            if (end >= hi) s_flag[1] = ord + g1 - 1;
+                        } else {
+                            for (int g = max(g0, first + seg0 - ord); g < min(g1, first + seg0 + A8_SEGS - ord); ++g) {
+                                const long long from = at + (long long)g * u, to = from + u;
+                                Seg x;
+                                x.b = b;
+                                x.g = g;
+                                x.tok = start + s.tok;
+                                x.rem = s.rem;
+                                x.rows = s.rows;
+                                x.pos = ctx - n + s.tok;
+                                x.page = s.page + (int)(max(from, lo) - from);
+                                x.pend = s.pend;
+                                x.v = (int)(max(from, lo) - lo);
+                                x.n = (int)(min(to, hi) - max(from, lo));
+                                x.c0 = (int)blockIdx.x - (from >= lo ? 0 : (int)((unsigned)(lo - from + per - 1) / (unsigned)per));
+                                x.c1 = (int)blockIdx.x + (to <= hi ? 0 : (int)((unsigned)(to - 1 - lo) / (unsigned)per));
+                                segs[ord + g - first - seg0] = x;
+                            }
+                        }
+                    }
+                    at = end;
+                    ord += p.G;
                 }
-                ++i;
-            });
+            }
         }
         __syncthreads();
+        if (seg0 < 0) {
+            first = s_flag[0];
+            nspans = s_flag[1] - first + 1;
+            continue;
+        }
         const int nseg = min(A8_SEGS, nspans - seg0);
         const int v0 = segs[0].v, v1 = segs[nseg - 1].v + segs[nseg - 1].n;
         const int nk = (v1 - v0 - part + nparts - 1) / nparts;  // pages of this part
 
-        // lane i of a batch: block id (-1: nothing to read) and scale exponents of page 32 * batch + i
-        int bid = -1, bid2 = -1, sc = 0, sc2 = 0;
-        const auto fetch = [&](int batch, int& id, int& e) {
+        // lane i of a batch: block id (-1: nothing to read), head, scale bytes of page 32 * batch + i
+        int bid = -1, bid2 = -1, gk = 0, gk2 = 0;
+        uint32_t kb = 0, kb2 = 0, vb = 0, vb2 = 0;
+        const auto fetch = [&](int batch, int& id, int& g, uint32_t& k_byte, uint32_t& v_byte) {
             const int k = batch * 32 + lane;
             id = -1;
-            e = 0;
             if (k >= nk) return;
             const int v = v0 + part + nparts * k;
             int a = 0, z = nseg - 1;  // the last span with segs[].v <= v
@@ -312,21 +358,21 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
             }
             const int page = segs[a].page + (v - segs[a].v);
             if (page >= segs[a].pend) return;
+            g = segs[a].g;
             id = p.tables[(size_t)segs[a].b * p.max_blocks + page];
             if (id < 0 || id >= p.num_blocks) {
                 raise_err(p.err, YK_DEV_ERR_BOUNDS);
                 id = -1;
                 return;
             }
-            const uint8_t* s = p.scales + (size_t)id * p.block_scales + p.layer_scale + segs[a].g;
-            e = (kv8_exponent(__ldg(s)) + 128) | (kv8_exponent(__ldg(s + p.G)) + 128) << 8 | segs[a].g << 16;
+            const uint8_t* s = p.scales + (size_t)id * p.block_scales + p.layer_scale + g;
+            k_byte = *s;
+            v_byte = s[p.G];
         };
-        fetch(0, bid, sc);
-        fetch(1, bid2, sc2);
         // page k of this part into its ring slot, once every warp of the part is done with the slot
         const auto issue = [&](int k, int base) {
             const int id = __shfl_sync(0xffffffffu, k - base < 32 ? bid : bid2, k & 31);
-            const int g = __shfl_sync(0xffffffffu, k - base < 32 ? sc : sc2, k & 31) >> 16;
+            const int g = __shfl_sync(0xffffffffu, k - base < 32 ? gk : gk2, k & 31);
             if (lane == 0 && !dead) {
                 const int kk = done + k, slot = kk & (depth - 1);
                 if (kk >= depth && !mbar_wait_bounded(empty + slot * 8, (uint32_t)((kk / depth - 1) & 1))) {
@@ -343,111 +389,105 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
             }
             dead = __shfl_sync(0xffffffffu, (int)dead, 0);
         };
+        fetch(0, bid, gk, kb, vb);
         if (rg == 0)
+#pragma unroll 1
             for (int k = 0; k < min(depth, nk); ++k) issue(k, 0);
+        fetch(1, bid2, gk2, kb2, vb2);
 
         int k = 0;
+#pragma unroll 1
         for (int si = 0; si < nseg; ++si) {
             const Seg sg = segs[si];
-            int start = p.q_starts[sg.b];
-            const int n = p.q_starts[sg.b + 1] - start, ctx = p.ctx[sg.b];
-            const int rows = (int)min((long long)R, (long long)n * rep - (long long)sg.qt * R);
-            const int row0 = sg.qt * R, my0 = rg * 8 * NT;  // first row of the tile, of this warp within it
-            const int pos_first = ctx - n + row0 / rep, pos_last = ctx - n + (row0 + rows - 1) / rep;
+            const int rows = sg.rows;
+            const int pos_last = sg.pos + div_rep(p, sg.rem + rows - 1);
             const bool active = my0 < rows;
+            // row i of the tile: token and query head of the group
+            const auto row_token = [&](int i) { return div_rep(p, sg.rem + i); };
 
-            // ---- queries: B fragments, column n = lane / 4, dims 64 h + 16 c + 4 s + {0, 1 | 2, 3}
-            uint32_t qf[C::QREG ? TERMS * NT * KS * 2 : 1];
-            const uint32_t q_smem = smem_u32(shared) + (uint32_t)(rg * TERMS * NT * KS * 256 + lane * 8);
-            float rf[NT][2];  // score of rows 2c, 2c + 1 -> log2 domain
-            if (active) {
+            // ---- queries to B fragments in shared memory, 8 rows at a time: column n = lane / 4,
+            // dims 64 h + 16 c + 4 s + {0, 1 | 2, 3} of k-step 4 h + s
+#pragma unroll 1
+            for (int u = warp; u * 8 < rows; u += 4) {
+                const int row = u * 8 + r, i = row_token(row);
+                const AT* src = reinterpret_cast<const AT*>(p.q) + (size_t)(sg.tok + i) * p.q_stride +
+                                (size_t)(sg.g * rep + sg.rem + row - i * rep) * DH + 16 * c;
+                float amax = 0.f;
+                uint4 w[sizeof(AT) == 2 ? NH * 2 : 1];
+                if constexpr (sizeof(AT) == 2) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const int row = my0 + nt * 8 + r, rr = row0 + row;
-                    const AT* src = reinterpret_cast<const AT*>(p.q) + (size_t)(start + rr / rep) * p.q_stride +
-                                    (size_t)(sg.g * rep + rr % rep) * DH + 16 * c;
-                    float amax = 0.f;
-                    uint32_t w[sizeof(AT) == 2 ? NH * 8 : 1];
-                    if constexpr (sizeof(AT) == 2) {
-#pragma unroll
-                        for (int h = 0; h < NH; ++h) {
-                            uint4 x = make_uint4(0, 0, 0, 0), y = x;
-                            if (row < rows) {
-                                x = __ldcg(reinterpret_cast<const uint4*>(src + 64 * h));
-                                y = __ldcg(reinterpret_cast<const uint4*>(src + 64 * h + 8));
-                            }
-                            const uint32_t t[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                w[h * 8 + i] = t[i];
-                                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[i] << 16)),
-                                                         fabsf(__uint_as_float(t[i] & 0xffff0000u))));
-                            }
-                        }
-                    } else {
-                        if (row < rows)
-#pragma unroll
-                            for (int h = 0; h < NH; ++h)
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(to_f32(src[64 * h + i])));
+                    for (int h = 0; h < NH * 2; ++h) {
+                        w[h] = make_uint4(0, 0, 0, 0);
+                        if (row < rows) w[h] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * (h >> 1)) + (h & 1));
                     }
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    // shift by 2^up: amax = m * 2^E, 1 <= m < 2, to m * 2^14
-                    const int E = (int)(__float_as_uint(amax) >> 23) - 127;
-                    const int up = amax == 0.f ? 0 : max(-100, min(100, 14 - E));
-                    const float f = exp2_int(up);
-                    const int down = -up;
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        rf[nt][j] = p.scale_log2 * exp2_int(__shfl_sync(0xffffffffu, down, 8 * c + 4 * j));
+                    for (int h = 0; h < NH * 2; ++h) {
+                        const uint32_t t[4] = {w[h].x, w[h].y, w[h].z, w[h].w};
 #pragma unroll
-                    for (int h = 0; h < NH; ++h)
+                        for (int z = 0; z < 4; ++z)
+                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[z] << 16)), fabsf(__uint_as_float(t[z] & 0xffff0000u))));
+                    }
+                } else if (row < rows) {
 #pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            float x[4];
-                            if constexpr (sizeof(AT) == 2) {
-                                const uint32_t a = w[h * 8 + 2 * s], b = w[h * 8 + 2 * s + 1];
-                                x[0] = __uint_as_float(a << 16);
-                                x[1] = __uint_as_float(a & 0xffff0000u);
-                                x[2] = __uint_as_float(b << 16);
-                                x[3] = __uint_as_float(b & 0xffff0000u);
-                            } else {
-                                float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if (row < rows) t = __ldcg(reinterpret_cast<const float4*>(src + 64 * h + 4 * s));
-                                x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
-                            }
+                    for (int h = 0; h < NH * 4; ++h) {
+                        const float4 t = __ldcg(reinterpret_cast<const float4*>(src + 64 * (h >> 2)) + (h & 3));
+                        amax = fmaxf(fmaxf(fmaxf(amax, fabsf(t.x)), fmaxf(fabsf(t.y), fabsf(t.z))), fabsf(t.w));
+                    }
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // shift by 2^up: amax = m * 2^E, 1 <= m < 2, to m * 2^14
+                const int up = amax == 0.f ? 0 : max(-100, min(100, 14 + 127 - (int)(__float_as_uint(amax) >> 23)));
+                const float f = exp2_int(up);
+                if (c == 0) s_rf[row] = p.scale_log2 * exp2_int(-up);
+                const uint32_t dst = smem_u32(shared) + (uint32_t)(u * TERMS * KS * 256 + lane * 16);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) x[i] *= f;
-                            uint32_t hi2[2] = {pack_f16(x[0], x[1]), pack_f16(x[2], x[3])};
+                for (int ks = 0; ks < KS; ++ks) {
+                    float x[4];
+                    if constexpr (sizeof(AT) == 2) {
+                        const uint4 q = w[ks >> 1];
+                        const uint32_t a = ks & 1 ? q.z : q.x, b = ks & 1 ? q.w : q.y;
+                        x[0] = __uint_as_float(a << 16);
+                        x[1] = __uint_as_float(a & 0xffff0000u);
+                        x[2] = __uint_as_float(b << 16);
+                        x[3] = __uint_as_float(b & 0xffff0000u);
+                    } else {
+                        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (row < rows) t = __ldcg(reinterpret_cast<const float4*>(src + 64 * (ks >> 2)) + (ks & 3));
+                        x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+                    }
 #pragma unroll
-                            for (int t = 0; t < TERMS; ++t) {
-                                if (t == 1) {  // what the first term leaves
-                                    const float2 a = f32x2(hi2[0]), b = f32x2(hi2[1]);
-                                    hi2[0] = pack_f16(x[0] - a.x, x[1] - a.y);
-                                    hi2[1] = pack_f16(x[2] - b.x, x[3] - b.y);
-                                }
-                                const int ks = h * 4 + s;
-                                if constexpr (C::QREG) {
-                                    qf[((t * NT + nt) * KS + ks) * 2] = hi2[0];
-                                    qf[((t * NT + nt) * KS + ks) * 2 + 1] = hi2[1];
-                                } else if (part == 0) {
-                                    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(
-                                                     q_smem + (uint32_t)(((t * NT + nt) * KS + ks) * 256)),
-                                                 "r"(hi2[0]), "r"(hi2[1])
-                                                 : "memory");
-                                }
-                            }
+                    for (int z = 0; z < 4; ++z) x[z] *= f;
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+                        const uint32_t y0 = pack_f16(x[0], x[1]), y1 = pack_f16(x[2], x[3]);
+                        asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(
+                                         dst + (uint32_t)(t * KS * 256 + (ks >> 1) * 512 + (ks & 1) * 8)),
+                                     "r"(y0), "r"(y1)
+                                     : "memory");
+                        if (TERMS == 2) {  // what this term leaves
+                            const float2 a = f32x2(y0), b = f32x2(y1);
+                            x[0] -= a.x; x[1] -= a.y; x[2] -= b.x; x[3] -= b.y;
                         }
+                    }
                 }
             }
-            if constexpr (!C::QREG) __syncthreads();
+            __syncthreads();
+            const uint32_t q_smem = smem_u32(shared) + (uint32_t)(rg * NT * TERMS * KS * 256 + lane * 16);
+            uint4 qf[C::QREG ? NT * TERMS * KS / 2 : 1];
+            if constexpr (C::QREG) {
+                if (active)
+#pragma unroll
+                    for (int i = 0; i < NT * TERMS * KS / 2; ++i) qf[i] = lds128(q_smem + i * 512);
+            }
+            float2 rf[NT];  // scores of rows 2c, 2c + 1 -> log2 domain
 
             float o[MT][NT][4];
             float m[NT][2], l[NT][2];  // m: the row's reference, less the bias of 7
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                m[nt][0] = m[nt][1] = -3.402823466e38f;
+                rf[nt] = *reinterpret_cast<const float2*>(s_rf + my0 + nt * 8 + 2 * c);
+                m[nt][0] = m[nt][1] = LOWEST;
                 l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
                 for (int t = 0; t < MT; ++t) o[t][nt][0] = o[t][nt][1] = o[t][nt][2] = o[t][nt][3] = 0.f;
@@ -455,17 +495,21 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
 
             // ---- this part's pages of the span
             const int v_end = sg.v + sg.n;
+#pragma unroll 1
             for (; k < nk && v0 + part + nparts * k < v_end; ++k) {
                 const int base = k & ~31;
                 if (k == base && k > 0) {
                     bid = bid2;
-                    sc = sc2;
-                    fetch(k / 32 + 1, bid2, sc2);
+                    gk = gk2;
+                    kb = kb2;
+                    vb = vb2;
+                    fetch(k / 32 + 1, bid2, gk2, kb2, vb2);
                 }
                 if (rg == 0 && k > 0 && k - 1 + depth < nk) issue(k - 1 + depth, base);
                 const int kk = done + k, slot = kk & (depth - 1);
                 const int id = __shfl_sync(0xffffffffu, bid, k & 31);
-                const int e = __shfl_sync(0xffffffffu, sc, k & 31);
+                const int ek = kv8_exponent(__shfl_sync(0xffffffffu, kb, k & 31));
+                const int ev = kv8_exponent(__shfl_sync(0xffffffffu, vb, k & 31));
                 if (!dead && !mbar_wait_bounded(full + slot * 8, (uint32_t)(kk / depth & 1))) {
                     if (lane == 0) raise_err(p.err, YK_DEV_ERR_TIMEOUT);
                     dead = true;
@@ -483,46 +527,51 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
                         const uint4 x4 = lds128(ka), y4 = lds128(ka + 8 * C::ROWB);
                         const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t a[4] = {f16x2_lo(x[i]), f16x2_lo(y[i]), f16x2_hi(x[i]), f16x2_hi(y[i])};
-                            const int ks = h * 4 + i;
+                        for (int i = 0; i < 4; i += 2) {
+                            const uint32_t a0[4] = {f16x2_lo(x[i]), f16x2_lo(y[i]), f16x2_hi(x[i]), f16x2_hi(y[i])};
+                            const uint32_t a1[4] = {f16x2_lo(x[i + 1]), f16x2_lo(y[i + 1]), f16x2_hi(x[i + 1]), f16x2_hi(y[i + 1])};
 #pragma unroll
-                            for (int t = 0; t < TERMS; ++t)
+                            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    if constexpr (C::QREG) {
-                                        mma_f16(s[nt], a, qf[((t * NT + nt) * KS + ks) * 2], qf[((t * NT + nt) * KS + ks) * 2 + 1]);
-                                    } else {
-                                        const uint2 b = lds64(q_smem + (uint32_t)(((t * NT + nt) * KS + ks) * 256));
-                                        mma_f16(s[nt], a, b.x, b.y);
-                                    }
+                                for (int t = 0; t < TERMS; ++t) {
+                                    const int at = ((nt * TERMS + t) * KS + h * 4 + i) / 2;
+                                    const uint4 b = C::QREG ? qf[C::QREG ? at : 0] : lds128(q_smem + at * 512);
+                                    mma_f16(s[nt], a0, b.x, b.y);
+                                    mma_f16(s[nt], a1, b.z, b.w);
                                 }
                         }
                     }
                     // scores -> x + e_V in the log2 domain; row 2c: s[0], s[2], row 2c + 1: s[1], s[3]
-                    const int ek = (e & 255) - 128, ev = (e >> 8 & 255) - 128;
                     const float fk = exp2_int(ek), shift = (float)ev, inv = exp2_int(-ev);
-                    const bool plain = p.cap <= 0.f && j0 + 15 <= pos_first && (p.window <= 0 || pos_last - j0 < p.window);
-                    uint32_t seen = 0xffffffffu;  // bit nt * 4 + i: s[nt][i]'s key is visible to its row
+                    const bool plain = p.cap <= 0.f && j0 + 15 <= sg.pos && (p.window <= 0 || pos_last - j0 < p.window);
                     if (plain) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                s[nt][i] = fmaf(s[nt][i], fminf(rf[nt][i & 1] * fk, 3.402823466e38f), shift);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const float f0 = fminf(rf[nt].x * fk, LARGEST), f1 = fminf(rf[nt].y * fk, LARGEST);
+                            s[nt][0] = fmaf(s[nt][0], f0, shift);
+                            s[nt][1] = fmaf(s[nt][1], f1, shift);
+                            s[nt][2] = fmaf(s[nt][2], f0, shift);
+                            s[nt][3] = fmaf(s[nt][3], f1, shift);
+                        }
                     } else {
-                        seen = 0;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int row = my0 + nt * 8 + 2 * c + (i & 1);
-                                const int pos = ctx - n + (row0 + row) / rep, j = j0 + sigma + (i >> 1) * 8;
-                                const bool vis = row < rows && j <= pos && (p.window <= 0 || pos - j < p.window);
-                                float x = s[nt][i] * fminf(rf[nt][i & 1] * fk, 3.402823466e38f);
-                                if (p.cap > 0.f) x = p.cap_log2 * tanhf(x * p.inv_cap_log2);
-                                s[nt][i] = vis ? x + shift : -INFINITY;
-                                seen |= (vis ? 1u : 0u) << (nt * 4 + i);
+                            for (int i = 0; i < 4; ++i) s[nt][i] *= fminf((i & 1 ? rf[nt].y : rf[nt].x) * fk, LARGEST);
+                        if (p.cap > 0.f)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) s[nt][i] = p.cap_log2 * tanh_cap(s[nt][i] * p.inv_cap_log2);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const int row = my0 + nt * 8 + 2 * c + j;
+                                const int back = sg.pos + row_token(row) - (j0 + sigma);  // query minus first key
+                                const unsigned w = row < rows ? (p.window > 0 ? (unsigned)p.window : 0x80000000u) : 0u;
+                                s[nt][j] = (unsigned)back < w ? s[nt][j] + shift : -INFINITY;
+                                s[nt][j + 2] = (unsigned)(back - 8) < w ? s[nt][j + 2] + shift : -INFINITY;
                             }
                     }
                     // raise a row's reference once a weight would pass 2^15
@@ -571,23 +620,53 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
                     for (int bx = 0; bx < C::BOXES; ++bx) {
                         constexpr int W = DH == 64 ? 2 : 4;  // words of a thread's V bytes per key
                         uint32_t v[4][W];
-                        bool nan = false;
+                        const uint32_t va = page + (uint32_t)(bx * C::BOX);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const uint32_t va = page + (uint32_t)(bx * C::BOX + (j >> 1) * 8 * C::ROWB) + v_off[j & 1];
+                            const uint32_t a = va + (uint32_t)((j >> 1) * 8 * C::ROWB) + v_off[j & 1];
                             if constexpr (DH == 64) {
-                                const uint2 t = lds64(va);
+                                const uint2 t = lds64(a);
                                 v[j][0] = t.x; v[j][1] = t.y;
                             } else {
-                                const uint4 t = lds128(va);
+                                const uint4 t = lds128(a);
                                 v[j][0] = t.x; v[j][1] = t.y; v[j][2] = t.z; v[j][3] = t.w;
                             }
-                            if (!plain)
-#pragma unroll
-                                for (int i = 0; i < W; ++i)
-                                    nan |= ((v[j][i] & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u) != 0;
                         }
-                        nan = !plain && __any_sync(0xffffffffu, nan);
+                        if (!plain) {
+                            // a NaN cell must reach the rows that see its key and no others: it is taken
+                            // out of the product, and noted for the rows it belongs to
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                for (int i = 0; i < W; ++i) any |= (v[j][i] & 0x7f7f7f7fu) + 0x01010101u;
+                            if (any & 0x80808080u) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                    for (int i = 0; i < W; ++i) {
+                                        const uint32_t bad = ((v[j][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                        v[j][i] &= ~(bad | (bad - (bad >> 7)));
+                                    }
+#pragma unroll 1
+                                for (int z = 0; z < 16 * W; ++z) {
+                                    const int key = c + 4 * (z / (4 * W)), byte = z % (4 * W);
+                                    uint32_t x;
+                                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(
+                                        va + (uint32_t)((key >> 3) * 8 * C::ROWB) + v_off[key >> 2 & 1] + (uint32_t)byte));
+                                    if ((x & 0x7f) != 0x7f) continue;
+                                    const int dim = bx * 128 + v_dim + byte;
+                                    for (int row = my0; row < min(rows, my0 + C::ROWS); ++row) {
+                                        const int back = sg.pos + row_token(row) - (j0 + key);
+                                        if (back >= 0 && (p.window <= 0 || back < p.window)) {
+                                            atomicOr(&s_nan[row * (DH / 32) + (dim >> 5)], 1u << (dim & 31));
+                                            s_flag[3] = 1;
+                                        }
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                        }
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
                             const uint32_t lo01 = __byte_perm(v[0][i], v[1][i], 0x5140), hi01 = __byte_perm(v[0][i], v[1][i], 0x7362);
@@ -595,29 +674,8 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
 #pragma unroll
                             for (int half = 0; half < 2; ++half) {
                                 const uint32_t w0 = half ? hi01 : lo01, w1 = half ? hi23 : lo23;
-                                uint32_t a[4] = {f16x2_lo(w0), f16x2_hi(w0), f16x2_lo(w1), f16x2_hi(w1)};
+                                const uint32_t a[4] = {f16x2_lo(w0), f16x2_hi(w0), f16x2_lo(w1), f16x2_hi(w1)};
                                 const int t = bx * 8 + 2 * i + half;
-                                if (nan) {
-                                    // a NaN cell reaches the rows that see its key, and no others: it counts as 0
-                                    // here, and rows with a visible one become NaN (a product of flags finds them)
-                                    uint32_t flag[4];
-#pragma unroll
-                                    for (int z = 0; z < 4; ++z) {
-                                        const uint32_t bad = __hneu2_mask(*reinterpret_cast<__half2*>(&a[z]), *reinterpret_cast<__half2*>(&a[z]));
-                                        flag[z] = bad & 0x3c003c00u;  // 1.0
-                                        a[z] &= ~bad;
-                                    }
-#pragma unroll
-                                    for (int nt = 0; nt < NT; ++nt) {
-                                        float hit[4] = {0.f, 0.f, 0.f, 0.f};
-                                        const uint32_t f0 = (seen >> (nt * 4) & 1) * 0x3c00u | (seen >> (nt * 4 + 1) & 1) * 0x3c000000u;
-                                        const uint32_t f1 = (seen >> (nt * 4 + 2) & 1) * 0x3c00u | (seen >> (nt * 4 + 3) & 1) * 0x3c000000u;
-                                        mma_f16(hit, flag, transpose8(f0), transpose8(f1));
-#pragma unroll
-                                        for (int z = 0; z < 4; ++z)
-                                            if (hit[z] > 0.f) o[t][nt][z] = __int_as_float(0x7fffffff);
-                                    }
-                                }
 #pragma unroll
                                 for (int tm = 0; tm < TERMS; ++tm)
 #pragma unroll
@@ -630,7 +688,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
                 if (lane == 0) mbar_arrive(empty + slot * 8);
             }
 
-            // ---- end of the span: the parts of a row group are joined
+            // ---- end of the span: the parts of a row group are joined in shared memory
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -638,137 +696,127 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS_PER_SM)
                     l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
                     l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
                     l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
-                    if (r == 0) s_ml[warp * 8 * NT + nt * 8 + 2 * c + j] = make_float2(m[nt][j], l[nt][j]);
+                    if (r == 0) s_ml[warp * C::ROWS + nt * 8 + 2 * c + j] = make_float2(m[nt][j], l[nt][j]);
                 }
             __syncthreads();  // (and every warp is done with the queries in `shared`)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int at = nt * 8 + 2 * c + j;
-                    float M = -3.402823466e38f, L = 0.f;
-                    for (int q = 0; q < nparts; ++q) M = fmaxf(M, s_ml[((q << p.lg) + rg) * 8 * NT + at].x);
-                    for (int q = 0; q < nparts; ++q) {
-                        const float2 t = s_ml[((q << p.lg) + rg) * 8 * NT + at];
-                        L += t.y * ex2(t.x - M);
-                    }
-                    const float f = ex2(m[nt][j] - M);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        o[t][nt][j] *= f;
-                        o[t][nt][j + 2] *= f;
-                    }
-                    m[nt][j] = M;
-                    l[nt][j] = L;
+            if ((int)threadIdx.x < rows) {
+                const int row = threadIdx.x, w0 = row >= C::ROWS ? 1 : 0;  // (w0: the row group)
+                float M = LOWEST, L = 0.f;
+                for (int q = 0; q < nparts; ++q) M = fmaxf(M, s_ml[((q << p.lg) + w0) * C::ROWS + row - w0 * C::ROWS].x);
+                for (int q = 0; q < nparts; ++q) {
+                    const float2 t = s_ml[((q << p.lg) + w0) * C::ROWS + row - w0 * C::ROWS];
+                    L += t.y * ex2(t.x - M);
                 }
-            // warps 2, 3 -> 0, 1 (their row group's part with the same index mod 2); then, with four
-            // parts, 0 and 1 swap halves so that both finish half of the dims
-            float4* const dump = reinterpret_cast<float4*>(shared);  // [2 warps][MT][NT][32 lanes]
-            if (warp >= 2) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
+                s_row[row] = make_float2(M, L);
+            }
+            __syncthreads();
+            // warps 0, 1 write, 2, 3 add: buffer warp & 1 (its row group, or half of the parts)
+#pragma unroll 1
+            for (int turn = 0; turn < 2; ++turn) {
+                if (warp >> 1 == turn && active) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        dump[(((warp - 2) * MT + t) * NT + nt) * 32 + lane] = make_float4(o[t][nt][0], o[t][nt][1], o[t][nt][2], o[t][nt][3]);
-            }
-            __syncthreads();
-            if (warp < 2) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        const float4 x = dump[((warp * MT + t) * NT + nt) * 32 + lane];
-                        o[t][nt][0] += x.x; o[t][nt][1] += x.y; o[t][nt][2] += x.z; o[t][nt][3] += x.w;
-                    }
-            }
-            int t0 = 0, t1 = MT;  // the m-tiles this warp finishes
-            if (RG == 1) {
-                __syncthreads();
-                if (warp < 2) {
-#pragma unroll
-                    for (int t = 0; t < MT; ++t)
-                        if ((t >= MT / 2) == (warp == 0))
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                dump[(t * NT + nt) * 32 + lane] = make_float4(o[t][nt][0], o[t][nt][1], o[t][nt][2], o[t][nt][3]);
-                }
-                __syncthreads();
-                if (warp < 2) {
-#pragma unroll
-                    for (int t = 0; t < MT; ++t)
-                        if ((t >= MT / 2) == (warp == 1))
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const float4 x = dump[(t * NT + nt) * 32 + lane];
-                                o[t][nt][0] += x.x; o[t][nt][1] += x.y; o[t][nt][2] += x.z; o[t][nt][3] += x.w;
-                            }
-                    t0 = warp * (MT / 2);
-                    t1 = t0 + MT / 2;
-                }
-            }
-            const bool whole = sg.c0 == sg.c1;
-            const int mine_slot = 2 * (int)blockIdx.x + ((int)blockIdx.x == sg.c0 ? 1 : 0);
-            if (warp < 2 && active) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int row = my0 + nt * 8 + 2 * c + j, rr = row0 + row;
-                        if (row < rows) {
-                            const float z = whole ? (l[nt][j] == 0.f ? 0.f : 1.0f / l[nt][j]) : 1.f;
-                            AT* dst = reinterpret_cast<AT*>(p.out) + (size_t)(start + rr / rep) * p.out_stride +
-                                      (size_t)(sg.g * rep + rr % rep) * DH;
-                            float* ws = p.ws_o + ((size_t)mine_slot * R + row) * DH;
-                            if (!whole && r == 0 && t0 == 0)
-                                __stcg(p.ws_ml + (size_t)mine_slot * R + row, make_float2(m[nt][j], l[nt][j]));
+                        for (int j = 0; j < 2; ++j) {
+                            const int row = nt * 8 + 2 * c + j;
+                            const float f = ex2(m[nt][j] - s_row[my0 + row].x);
+                            float* const dst = s_o + ((warp & 1) * C::ROWS + row) * C::LDO + v_dim;
 #pragma unroll
                             for (int t = 0; t < MT; t += 2) {  // 4 consecutive dims
-                                if (t < t0 || t >= t1) continue;
-                                const int d = (t >> 3) * 128 + v_dim + 2 * (t & 7);
-                                const float a0 = o[t][nt][j] * z, a1 = o[t][nt][j + 2] * z;
-                                const float a2 = o[t + 1][nt][j] * z, a3 = o[t + 1][nt][j + 2] * z;
-                                if (whole) store4(dst + d, a0, a1, a2, a3);
-                                else __stcg(reinterpret_cast<float4*>(ws + d), make_float4(a0, a1, a2, a3));
+                                float4* const d = reinterpret_cast<float4*>(dst + (t >> 3) * 128 + 2 * (t & 7));
+                                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (turn) x = *d;
+                                x.x = fmaf(o[t][nt][j], f, x.x);
+                                x.y = fmaf(o[t][nt][j + 2], f, x.y);
+                                x.z = fmaf(o[t + 1][nt][j], f, x.z);
+                                x.w = fmaf(o[t + 1][nt][j + 2], f, x.w);
+                                *d = x;
                             }
                         }
-                    }
-            }
-            if (whole) {
-                __syncthreads();  // `shared` and s_ml are free again
-                continue;
-            }
-            // ---- a span cut across CTAs: the last of them to finish joins the parts, in order
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) s_flag[0] = atomicAdd(&p.counters[sg.c0], 1) == sg.c1 - sg.c0;
-            __syncthreads();
-            if (s_flag[0]) {
-                __threadfence();
-                constexpr int D4 = DH / 4;
-                for (int i = threadIdx.x; i < rows * D4; i += A8_THREADS) {
-                    const int row = i / D4, d = i % D4 * 4;
-                    float M = -3.402823466e38f, L = 0.f;
-                    for (int q = sg.c0; q <= sg.c1; ++q)
-                        M = fmaxf(M, __ldcg(p.ws_ml + (size_t)(2 * q + (q == sg.c0)) * R + row).x);
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int q = sg.c0; q <= sg.c1; ++q) {
-                        const size_t at = (size_t)(2 * q + (q == sg.c0)) * R + row;
-                        const float2 t = __ldcg(p.ws_ml + at);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * DH + d));
-                        const float f = ex2(t.x - M);
-                        L += t.y * f;
-                        a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
-                    }
-                    const float z = L == 0.f ? 0.f : 1.0f / L;
-                    const int rr = row0 + row;
-                    store4(reinterpret_cast<AT*>(p.out) + (size_t)(start + rr / rep) * p.out_stride +
-                               (size_t)(sg.g * rep + rr % rep) * DH + d, a.x * z, a.y * z, a.z * z, a.w * z);
                 }
-                if (threadIdx.x == 0) p.counters[sg.c0] = 0;
+                __syncthreads();
             }
-            __syncthreads();
+            const bool whole = sg.c0 == sg.c1, nans = s_flag[3] != 0;
+            const size_t part_row = (size_t)(2 * blockIdx.x + ((int)blockIdx.x == sg.c0 ? 1 : 0)) * R;
+#pragma unroll 1
+            for (int i = threadIdx.x; i < rows * D4; i += A8_THREADS) {
+                const int row = i / D4, d = i % D4 * 4;
+                float4 x = *reinterpret_cast<const float4*>(s_o + row * C::LDO + d);
+                if (RG == 1) {
+                    const float4 y = *reinterpret_cast<const float4*>(s_o + (C::ROWS + row) * C::LDO + d);
+                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                }
+                if (nans) {
+                    const uint32_t bad = s_nan[row * (DH / 32) + (d >> 5)] >> (d & 31);
+                    const float nan = __int_as_float(0x7fffffff);
+                    if (bad & 1) x.x = nan;
+                    if (bad & 2) x.y = nan;
+                    if (bad & 4) x.z = nan;
+                    if (bad & 8) x.w = nan;
+                }
+                const float2 ml = s_row[row];
+                if (whole) {
+                    const float z = ml.y == 0.f ? 0.f : 1.0f / ml.y;
+                    const int tok = row_token(row);
+                    store4(reinterpret_cast<AT*>(p.out) + (size_t)(sg.tok + tok) * p.out_stride +
+                               (size_t)(sg.g * rep + sg.rem + row - tok * rep) * DH + d, x.x * z, x.y * z, x.z * z, x.w * z);
+                } else {
+                    __stcg(reinterpret_cast<float4*>(p.ws_o + (part_row + row) * DH + d), x);
+                    if (d == 0) __stcg(p.ws_ml + part_row + row, ml);
+                }
+            }
+            if (nans) {
+                __syncthreads();
+                for (int i = threadIdx.x; i < C::NANS / 4; i += A8_THREADS) s_nan[i] = 0;
+                if (threadIdx.x == 0) s_flag[3] = 0;
+            }
+            if (!whole) {
+                // ---- a span cut across CTAs: the last of them to finish joins the parts, in order
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) s_flag[2] = atomicAdd(&p.counters[sg.c0], 1) == sg.c1 - sg.c0;
+                __syncthreads();
+                if (s_flag[2]) {
+                    __threadfence();
+                    const int nq = sg.c1 - sg.c0 + 1;
+                    const auto from = [&](int q) { return (size_t)(2 * (sg.c0 + q) + (q == 0)) * R; };
+                    if ((int)threadIdx.x < rows) {
+                        const int row = threadIdx.x;
+                        float M = LOWEST, L = 0.f;
+#pragma unroll 8
+                        for (int q = 0; q < nq; ++q) {  // (no branch: the loads go out together)
+                            const float2 t = __ldcg(p.ws_ml + from(q) + row);
+                            const float mn = fmaxf(M, t.x);
+                            L = fmaf(L, ex2(M - mn), t.y * ex2(t.x - mn));
+                            M = mn;
+                        }
+                        s_row[row] = make_float2(M, L == 0.f ? 0.f : 1.0f / L);
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int i = threadIdx.x; i < rows * D4; i += A8_THREADS) {
+                        const int row = i / D4, d = i % D4 * 4;
+                        const float2 M = s_row[row];
+                        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                        for (int q = 0; q < nq; ++q) {
+                            const size_t at = from(q) + row;
+                            const float f = ex2(__ldcg(&p.ws_ml[at].x) - M.x);
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * DH + d));
+                            a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
+                        }
+                        const int tok = row_token(row);
+                        store4(reinterpret_cast<AT*>(p.out) + (size_t)(sg.tok + tok) * p.out_stride +
+                                   (size_t)(sg.g * rep + sg.rem + row - tok * rep) * DH + d,
+                               a.x * M.y, a.y * M.y, a.z * M.y, a.w * M.y);
+                    }
+                    if (threadIdx.x == 0) p.counters[sg.c0] = 0;
+                }
+            }
+            __syncthreads();  // `shared` and the rows' values are free again
         }
         done += nk;
+        __syncthreads();  // (the span list too)
     }
     // every copy asked for has landed: the loop above waited for each, unless it gave up
     if (dead && rg == 0 && lane == 0)
@@ -830,6 +878,7 @@ yk_status attention_e4m3_check(const yk_attention_e4m3_args& a) {
     YK_ARG(a.T >= 0 && a.B > 0 && a.B <= (1 << 20), "T must not be negative, B in 1..2^20");
     YK_ARG(a.n_heads > 0 && a.n_heads <= 65536 && a.n_heads % a.pages.n_kv_heads == 0,
            "n_heads must be a positive multiple of n_kv_heads");
+    YK_ARG(a.n_heads / a.pages.n_kv_heads <= 1024, "at most 1024 query heads share a KV head");
     YK_ARG(a.max_blocks > 0 && a.max_blocks <= (1 << 27), "max_blocks must be in 1..2^27");
     YK_ARG(a.max_new >= 0 && a.window >= 0, "max_new / window must not be negative");
     YK_ARG(std::isfinite(a.scale) && a.scale >= 0.f && std::isfinite(a.cap) && a.cap >= 0.f,
@@ -841,7 +890,14 @@ yk_status attention_e4m3_check(const yk_attention_e4m3_args& a) {
     const int64_t es = a.dtype == YK_DTYPE_F32 ? 4 : 2, row = (int64_t)a.n_heads * a.pages.head_dim;
     YK_ARG(a.q_stride >= row && a.q_stride * es % 16 == 0 && a.out_stride >= row && a.out_stride * es % 16 == 0,
            "q_stride / out_stride must cover a row and be multiples of 16 bytes");
-    YK_ARG((int64_t)a.T * a.n_heads <= (int64_t)1 << 31, "T * n_heads too large");
+    // the kernel counts tiles (of 8 rows at least) and their pages in 31 and 38 bits
+    const int64_t rep = a.n_heads / a.pages.n_kv_heads, tiles = ((int64_t)a.T * rep / 8 + a.B) * a.pages.n_kv_heads;
+    if ((int64_t)a.T * a.n_heads > (int64_t)1 << 31 || tiles >= (int64_t)1 << 31 ||
+        (int64_t)a.pages.n_kv_heads * a.max_blocks >= (int64_t)1 << 31 ||
+        (double)tiles * a.max_blocks >= 274877906944.0) {
+        yk_set_error("unsupported: T, B, n_heads and max_blocks together are too large for one call");
+        return YK_ERR_UNSUPPORTED;
+    }
     return YK_OK;
 }
 
@@ -909,6 +965,10 @@ yk_status attention_e4m3_launch(cudaStream_t st, bool pdl, int num_sms, const yk
     p.cap_log2 = a.cap * log2e;
     p.inv_cap_log2 = a.cap > 0.f ? 1.0f / p.cap_log2 : 0.f;
     uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
+    const unsigned rep = (unsigned)(a.n_heads / a.pages.n_kv_heads);
+    p.rep_magic = rep == 1 ? 0u : (unsigned)((0x100000000ull + rep - 1) / rep);
+    const unsigned grid = (unsigned)(num_sms * A8_CTAS_PER_SM);
+    p.grid_magic = 0xffffffffffffffffull / grid + 1;
     const int dh = a.pages.head_dim;
     const size_t ws_rows = (size_t)16 * (dh == 256 ? 2 : 4) * 2 * A8_CTAS_PER_SM * num_sms;
     p.counters = reinterpret_cast<int32_t*>(ws);
