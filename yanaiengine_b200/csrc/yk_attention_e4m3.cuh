@@ -1,0 +1,281 @@
+// yk_attention_e4m3.cuh -- what the two kernels of yk_attention_e4m3 share: the
+// arguments, the division of the work over resident CTAs, the joining of spans
+// that were cut between CTAs.
+#pragma once
+#include "yk_epilogue.cuh"
+#include "yk_kvcache.cuh"
+
+namespace yk {
+
+constexpr int A8_SEGS = 32;        // spans a CTA lists at a time
+constexpr int A8_COUNTERS = 4096;  // bytes of arrival counters, one per CTA
+constexpr int A8_MIN_PAGES = 8;    // pages of a CTA's range, at least
+constexpr int A8_SCAN = 48;        // shared words of a8_plan
+constexpr float A8_LOWEST = -3.402823466e38f, A8_LARGEST = 3.402823466e38f;
+
+struct Attn8Params {
+    const void* q;
+    void* out;
+    const uint8_t* pool;
+    const uint8_t* scales;
+    const int32_t *q_starts, *ctx, *tables;
+    uint32_t* err;
+    int32_t* counters;  // workspace: arrivals at a cut span, by its first CTA (zero between calls)
+    float2* ws_ml;      // workspace: (m, l) and O of the parts of cut spans, [2 per CTA][R]
+    float* ws_o;
+    long long q_stride, out_stride;
+    long long block_scales, layer_scale, block_cells, layer_off;
+    int T, B, H, G, layer, max_blocks, num_blocks;
+    int lg;             // log2 of the row groups
+    uint32_t rep_magic;  // ceil(2^32 / (H / G)), 0 where that is 1
+    int window;
+    float scale_log2, cap, cap_log2, inv_cap_log2;  // _log2: times log2(e)
+};
+
+struct Seg {
+    int b, g;
+    int tok, rem;    // first row of the tile: token tok of the batch, query head rem of the group
+    int rows;
+    int pos;         // position of that token
+    int page, pend;  // first page of this CTA's part; pages of the span's keys end here
+    int v, n;        // its place and length (pages) in the CTA's range
+    int c0, c1;      // first and last CTA of the span
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// tanh to a few 2^-24 of its value: 1 - 2 / (1 + e^2z) away from 0, the odd
+// series z - z^3/3 + 2z^5/15 - 17z^7/315 near it.
+__device__ __forceinline__ float tanh_cap(float z) {
+    const float e = 1.f - __fdividef(2.f, 1.f + ex2(fminf(z * 2.8853900817779268f, 126.f)));
+    const float q = z * z, t = fmaf(fmaf(fmaf(-17.f / 315.f, q, 2.f / 15.f), q, -1.f / 3.f), q, 1.f) * z;
+    return fabsf(z) < 0.25f ? t : e;
+}
+
+// x / (H / G), x below 64 + H / G (exact: x * (H / G) < 2^32).
+__device__ __forceinline__ int div_rep(const Attn8Params& p, int x) {
+    return p.rep_magic ? (int)__umulhi((unsigned)x, p.rep_magic) : x;
+}
+
+// A span's pages: [page, pend), at least one (page == pend: a tile without keys).
+struct Span {
+    int rows, page, pend, tok, rem;  // tok: of the sequence
+    template <int PU>  // in units of PU pages
+    __device__ __forceinline__ int units() const { return max(1, (pend - page + PU - 1) / PU); }
+};
+__device__ __forceinline__ Span span_of(const Attn8Params& p, int n, int ctx, int qt, int R, int rep) {
+    const long long lo = (long long)qt * R;
+    Span s;
+    s.rows = (int)min((long long)n * rep - lo, (long long)R);
+    s.tok = qt == 0 ? 0 : (int)((unsigned)lo / (unsigned)rep);
+    s.rem = (int)lo - s.tok * rep;
+    const int first = ctx - n + s.tok;
+    const int last = first + div_rep(p, s.rem + s.rows - 1);
+    s.pend = (int)((min(max((long long)last + 1, 0LL), (long long)p.max_blocks * 16) + 15) >> 4);
+    s.page = p.window > 0 ? min(max(0, first - p.window + 1) >> 4, s.pend) : 0;
+    return s;
+}
+
+// New tokens of sequence b; 0 where q_starts does not fit.
+__device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& start) {
+    start = p.q_starts[b];
+    const int end = p.q_starts[b + 1];
+    return start >= 0 && end >= start && end <= p.T && (b > 0 || start == 0) ? end - start : -1;
+}
+
+
+// A thread's sequences and this CTA's range of units, [lo, hi) of the spans laid end to end.
+struct A8Work {
+    int b_lo, b_hi;
+    unsigned units, at0;  // of the thread's sequences, and before them
+    unsigned per, lo, hi;
+    int ord0;             // spans before the thread's
+    int first, nspans;    // spans of the range
+};
+
+// Block-wide: the range from the lengths on the device (prefix sums over the
+// sequences, THREADS threads).  False: nothing for this CTA.
+template <int THREADS, int PU>
+__device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, unsigned* s_scan, A8Work& w) {
+    constexpr int WARPS = THREADS / 32;
+    static_assert(2 * WARPS + 2 <= A8_SCAN, "scan words");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per_thread = (p.B + THREADS - 1) / THREADS;
+    w.b_lo = min(p.B, (int)threadIdx.x * per_thread);
+    w.b_hi = min(p.B, w.b_lo + per_thread);
+    w.units = 0;  // (the host sees to it that all pages together stay below 2^31)
+    int spans = 0;
+    for (int b = w.b_lo; b < w.b_hi; ++b) {
+        int start;
+        const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+        if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
+        for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+            w.units += (unsigned)(span_of(p, n, ctx, qt, R, rep).units<PU>() * p.G);
+            spans += p.G;
+        }
+    }
+    w.at0 = w.units;  // exclusive prefixes over the threads
+    w.ord0 = spans;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, w.at0, o);
+        const int y = __shfl_up_sync(0xffffffffu, w.ord0, o);
+        if (lane >= o) {
+            w.at0 += x;
+            w.ord0 += y;
+        }
+    }
+    if (lane == 31) {
+        s_scan[warp] = w.at0;
+        s_scan[WARPS + warp] = (unsigned)w.ord0;
+    }
+    __syncthreads();
+    unsigned total = 0;
+    w.at0 -= w.units;
+    w.ord0 -= spans;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        if (i < warp) {
+            w.at0 += s_scan[i];
+            w.ord0 += (int)s_scan[WARPS + i];
+        }
+        total += s_scan[i];
+    }
+    w.per = max((unsigned)(A8_MIN_PAGES / PU), (total + gridDim.x - 1) / gridDim.x);
+    w.lo = min(total, blockIdx.x * w.per);
+    w.hi = min(total, w.lo + w.per);
+    if (w.lo >= w.hi) return false;
+    // the first and the last span of the range: the threads that hold them say so
+    if (w.at0 < w.hi && w.at0 + w.units > w.lo && (w.at0 <= w.lo || w.at0 + w.units >= w.hi)) {
+        unsigned at = w.at0;
+        int ord = w.ord0;
+        for (int b = w.b_lo; b < w.b_hi; ++b) {
+            int start;
+            const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+            for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+                const unsigned u = (unsigned)span_of(p, n, ctx, qt, R, rep).units<PU>(), end = at + u * p.G;
+                if (at <= w.lo && end > w.lo) s_scan[2 * WARPS] = (unsigned)ord + (w.lo - at) / u;
+                if (at < w.hi && end >= w.hi) s_scan[2 * WARPS + 1] = (unsigned)ord + (w.hi - at - 1) / u;
+                at = end;
+                ord += p.G;
+            }
+        }
+    }
+    __syncthreads();
+    w.first = (int)s_scan[2 * WARPS];
+    w.nspans = (int)s_scan[2 * WARPS + 1] - w.first + 1;
+    return true;
+}
+
+// Block-wide: spans seg0 .. seg0 + A8_SEGS - 1 of the range into segs (a barrier must follow).
+template <int PU>
+__device__ __noinline__ void a8_list(const Attn8Params& p, int R, int rep, const A8Work& w, int seg0, Seg* segs) {
+    if (w.at0 >= w.hi || w.at0 + w.units <= w.lo) return;
+    unsigned at = w.at0;
+    int ord = w.ord0 - w.first - seg0;  // place in segs
+    for (int b = w.b_lo; b < w.b_hi; ++b) {
+        int start;
+        const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+        for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+            const Span s = span_of(p, n, ctx, qt, R, rep);
+            const unsigned u = (unsigned)s.units<PU>();
+            for (int g = max(0, -ord); g < min(p.G, A8_SEGS - ord); ++g) {
+                const unsigned from = at + g * u, to = from + u;
+                if (to <= w.lo || from >= w.hi) continue;
+                Seg x;
+                x.b = b;
+                x.g = g;
+                x.tok = start + s.tok;
+                x.rem = s.rem;
+                x.rows = s.rows;
+                x.pos = ctx - n + s.tok;
+                x.page = s.page + PU * (int)(max(from, w.lo) - from);
+                x.pend = s.pend;
+                x.v = (int)(max(from, w.lo) - w.lo);
+                x.n = (int)(min(to, w.hi) - max(from, w.lo));
+                x.c0 = (int)blockIdx.x - (from >= w.lo ? 0 : (int)((w.lo - from + w.per - 1) / w.per));
+                x.c1 = (int)blockIdx.x + (to <= w.hi ? 0 : (int)((to - 1 - w.lo) / w.per));
+                segs[ord + g] = x;
+            }
+            at += u * p.G;
+            ord += p.G;
+        }
+    }
+}
+
+// One thread, after a barrier that follows the writing of a cut span's part:
+// counts it; the CTA that counts last will join the span.
+__device__ __forceinline__ void a8_arrive(const Attn8Params& p, const Seg& sg, int* s_last, Seg* s_cut) {
+    int n;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n) : "l"(p.counters + sg.c0) : "memory");
+    const int which = (int)blockIdx.x == sg.c0;
+    s_last[which] = n == sg.c1 - sg.c0;
+    s_cut[which] = sg;
+}
+
+// Block-wide, at the end.
+template <typename AT, int DH, int THREADS>
+__device__ __forceinline__ void a8_join(const Attn8Params& p, int R, int rep, const int* s_last, const Seg* s_cut) {
+    constexpr int D4 = DH / 4;
+    // ---- spans cut across CTAs (this CTA's first, begun elsewhere, or its last): the last
+    // CTA to arrive joins the parts, in their order
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        if (!s_last[which]) continue;
+        const Seg sg = s_cut[which];
+        __threadfence();
+        const int nq = sg.c1 - sg.c0 + 1;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < sg.rows * D4; i += THREADS) {
+            const int row = i / D4, d = i % D4 * 4;
+            float M = A8_LOWEST, L = 0.f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int q0 = 0; q0 < nq; q0 += 8) {  // eight parts' loads go out together
+                float2 t[8];
+                float4 x[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    const int q = min(q0 + z, nq - 1);
+                    const size_t at = (size_t)(2 * (sg.c0 + q) + (q == 0)) * R + row;
+                    t[z] = __ldcg(p.ws_ml + at);
+                    x[z] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * DH + d));
+                }
+                float mn = M;
+#pragma unroll
+                for (int z = 0; z < 8; ++z) mn = fmaxf(mn, t[z].x);
+                const float g = ex2(M - mn);
+                a.x *= g; a.y *= g; a.z *= g; a.w *= g;
+                L *= g;
+                M = mn;
+#pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    if (q0 + z < nq) {
+                        const float f = ex2(t[z].x - mn);
+                        L = fmaf(t[z].y, f, L);
+                        a.x = fmaf(x[z].x, f, a.x); a.y = fmaf(x[z].y, f, a.y);
+                        a.z = fmaf(x[z].z, f, a.z); a.w = fmaf(x[z].w, f, a.w);
+                    }
+                }
+            }
+            const float z = L == 0.f ? 0.f : 1.0f / L;
+            const int tok = div_rep(p, sg.rem + row);
+            store4(reinterpret_cast<AT*>(p.out) + (size_t)(sg.tok + tok) * p.out_stride +
+                       (size_t)(sg.g * rep + sg.rem + row - tok * rep) * DH + d, a.x * z, a.y * z, a.z * z, a.w * z);
+        }
+        if (threadIdx.x == 0) p.counters[sg.c0] = 0;
+        __syncthreads();
+    }
+}
+
+// CTAs per SM * rows of a tile * head_dim: at most this, for every shape (the workspace's parts).
+constexpr int A8_WS = 16384;
+
+// bf16 queries (yk_attention_e4m3_tc.cu); map: boxes of 16 K rows.
+yk_status attention_e4m3_launch_bf16(cudaStream_t st, bool pdl, int num_sms, int head_dim, const CUtensorMap& map,
+                                     const Attn8Params& p, long long rows);
+
+}  // namespace yk

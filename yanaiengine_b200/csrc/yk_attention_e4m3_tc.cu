@@ -1,0 +1,900 @@
+// yk_attention_e4m3_tc.cu -- yk_attention_e4m3 for bf16 queries, on the
+// tcgen05 tensor cores.
+//
+// One CTA per SM, resident; each takes an equal range of 128-key tiles of the
+// spans (sequence, query tile, KV head) laid end to end, found from the lengths
+// on the device.  Its warps are a pipeline:
+//   producers  one warp for K, one for V (a warp issues a copy in about 85 cycles,
+//              whatever its size): table entries and scale bytes; K pages by TMA
+//              (128- or 64-byte swizzle), V pages by bulk copy, into rings of tiles
+//   queries    the next span's queries into e4m3 pairs
+//   MMA        S^T[128 keys x 2R] = K Q^T (kind::f8f6f4), O^T[dims x R] += V^T P^T
+//              (kind::f16), accumulators in TMEM, S^T and O^T double-buffered
+//   softmax    8 warps, one key and half of the rows a thread: scores from TMEM,
+//              weights to shared memory
+//   V          4 warps: e4m3 V to f16, still [key][dim] (the MN-major operand of
+//              O^T); at a span's end they read O^T and write the result
+// K goes to the tensor core as it lies in the cache: no conversion at all.  The
+// queries, as bf16, are 8 bits wide: two e4m3 terms, the second scaled by 16,
+// hold them exactly (to 2^-21 of a row's largest value at least), as separate
+// columns of one product.  V converts once for all rows of the tile (R up to 64).
+//
+// Weights as in the other kernel: p = 2^(x + e_V - m), f16 with room for 2^8
+// before the reference m moves; m is common to the CTA, kept lazily: it moves
+// when a weight would pass 2^15, and at a span's first keys.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <string>
+
+#include "yk_attention_e4m3.cuh"
+
+namespace yk {
+
+constexpr int TCA_THREADS = 512;  // warps 0-7 softmax, 8-11 V, 12 K and 13 V copies, 14 MMA, 15 queries
+constexpr int TCA_TILE = 128;     // keys
+constexpr int TCA_PAGES = TCA_TILE / YK_BLOCK_SIZE;
+
+template <int DH, int RN>
+struct TcaCfg {
+    static constexpr int R = 8 * RN, RP = R <= 16 ? 16 : R <= 32 ? 32 : 64;  // rows; columns of O^T
+    static constexpr int RH = R / 2;                           // rows of a softmax thread
+    static constexpr int ROWB = DH == 64 ? 64 : 128;           // bytes of a K row in one TMA box
+    static constexpr int BOXES = DH / ROWB;
+    static constexpr int HALVES = DH == 256 ? 2 : 1;           // 128-dim products of O^T
+    static constexpr int KT = TCA_TILE * DH;                   // bytes of a K (or V) tile
+    static constexpr int NV16 = DH == 256 ? 1 : 2, V16 = 2 * KT;
+    static constexpr int PROW = 2 * RP;                        // bytes of a key's weights
+    static constexpr int PB = PROW * TCA_TILE, QB = 2 * R * DH;
+    static constexpr int INFO = 16;                            // tiles whose page words are kept
+    static constexpr int LDL = 33;
+    static constexpr int SMALL = 8 * 4 * LDL * 4 + (2 + 1 + 1 + 1 + 1 + 4 + 8 + 2 + 1 + 3) * R * 4 + R * (DH / 32) * 4 +
+                                 2 * INFO * TCA_PAGES * 4 + (A8_SEGS + 2) * (int)sizeof(Seg) + A8_SCAN * 4 + 64 * 8 + 128;
+    static constexpr int ROOM = 227 * 1024 - 1024 - SMALL - NV16 * V16 - 2 * PB - 2 * QB;
+    static constexpr int TILES = ROOM / KT;                    // K and V tiles that fit
+    static constexpr int NV = TILES / 2 < 6 ? TILES / 2 : 6, NK = TILES - NV < 6 ? TILES - NV : 6;
+    static constexpr int SMEM = 1024 + (NK + NV) * KT + NV16 * V16 + 2 * PB + 2 * QB + SMALL;
+    static constexpr int S_COLS = 2 * R, O_COLS = HALVES * RP;
+    static constexpr int COLS = 2 * S_COLS + 2 * O_COLS;
+    static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+    static_assert(NK >= 2 && NV >= 1 && COLS <= 512, "tile shapes");
+};
+
+// ---------------------------------------------------------------------------
+// Small wrappers.
+// ---------------------------------------------------------------------------
+// N columns of this thread's TMEM lane (the values are there after tmem_wait_ld).
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t* r) {
+    if constexpr (N >= 16) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(a));
+        if constexpr (N > 16) tmem_ld<N - 16>(a + 16, r + 16);
+    } else if constexpr (N >= 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(a));
+        if constexpr (N > 8) tmem_ld<N - 8>(a + 8, r + 8);
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(a));
+    }
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Shared-memory matrix descriptors (sm_100), as two words: the low one holds the
+// address and the leading stride, the high one the other stride and the swizzle
+// (2: 128 B, 4: 64 B, 6: 32 B).
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle) { return sbo >> 4 | 1u << 14 | swizzle << 29; }
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo = 0) { return addr >> 4 | lbo >> 4 << 16; }
+template <bool F8>
+__device__ __forceinline__ void mma_tc(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+    if constexpr (F8)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %5, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi),
+            "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi),
+            "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// Barriers of the 8 softmax warps (true if any thread says so) and of the 4 V warps.
+__device__ __forceinline__ bool softmax_or(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void v_bar() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
+__device__ __forceinline__ float warp_fmax(float v) {  // (NaN is passed over)
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
+    asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+// The rare ends of a wait and of a NaN cell, kept out of line: the kernel's loops
+// have to stay in the instruction cache.
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, uint32_t* err) {
+    const bool ok = mbar_wait_bounded(bar, parity);
+    if (!ok) raise_err(err, YK_DEV_ERR_TIMEOUT);
+    return ok;
+}
+// Notes the NaN cells among the 16 of a key at `cells` (dims dim0 ..) for the rows that see it.
+__device__ __noinline__ void note_nans(uint32_t cells, int dim0, int key, int pos, int rem, uint32_t rep_magic, int rows,
+                                       int window, int words, uint32_t* s_nan, int* s_flag) {
+#pragma unroll 1
+    for (int z = 0; z < 16; ++z) {
+        uint32_t x;
+        asm volatile("ld.shared.u8 %0, [%1];" : "=r"(x) : "r"(cells + (uint32_t)z));
+        if ((x & 0x7f) != 0x7f) continue;
+#pragma unroll 1
+        for (int row = 0; row < rows; ++row) {
+            const int back = pos + (rep_magic ? (int)__umulhi((unsigned)(rem + row), rep_magic) : rem + row) - key;
+            if (back >= 0 && (window <= 0 || back < window)) {
+                atomicOr(&s_nan[row * words + ((dim0 + z) >> 5)], 1u << ((dim0 + z) & 31));
+                *s_flag = 1;
+            }
+        }
+    }
+}
+
+// A ring's next place: slot and the parity of its use.
+template <int N>
+struct Turn {
+    int slot = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+__device__ __forceinline__ float cap_score(const Attn8Params& p, float x) { return p.cap_log2 * tanh_cap(x * p.inv_cap_log2); }
+
+// Whether every row of the span's tile sees all keys j0 .. j0 + 127.
+__device__ __forceinline__ bool all_seen(const Attn8Params& p, const Seg& sg, int pos_last, int j0) {
+    return j0 + TCA_TILE - 1 <= sg.pos && (p.window <= 0 || pos_last - j0 < p.window);
+}
+
+template <int DH, int RN>
+__global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Attn8Params p) {
+    using C = TcaCfg<DH, RN>;
+    constexpr int R = C::R, RP = C::RP, NK = C::NK, NV = C::NV, NV16 = C::NV16;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const k_ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* const v_ring = k_ring + NK * C::KT;
+    uint8_t* const v16 = v_ring + NV * C::KT;
+    uint8_t* const s_p = v16 + NV16 * C::V16;
+    uint8_t* const s_q = s_p + 2 * C::PB;
+    float* const s_lt = reinterpret_cast<float*>(s_q + 2 * C::QB);  // [8 warps][4][LDL]
+    float* const s_rf = s_lt + 8 * 4 * C::LDL;                      // [2][R] score factors of a span's rows
+    float* const s_neg = s_rf + 2 * R;                              // [R] references, negated
+    int* const s_set = reinterpret_cast<int*>(s_neg + R);             // [R] a row has seen a key
+    float* const s_f = reinterpret_cast<float*>(s_set + R);         // [R] factor and ...
+    float* const s_dm = s_f + R;                                    // [R] ... step of a row's last move
+    float* const s_mx = s_dm + R;                                   // [4][R]
+    float* const s_l = s_mx + 4 * R;                                // [2][4][R] sums
+    float* const s_mo = s_l + 8 * R;                                // [2][R] references at a span's end
+    int* const s_pos = reinterpret_cast<int*>(s_mo + 2 * R);        // [R] positions, for the softmax warps
+    float* const s_inv = reinterpret_cast<float*>(s_pos + R);       // [R] 1 / sum and ...
+    long long* const s_off = reinterpret_cast<long long*>(s_inv + R);       // [R] ... place of a result row
+    uint32_t* const s_nan = reinterpret_cast<uint32_t*>(s_off + R);         // [R][DH / 32]
+    // [2][INFO][8]: exponents of a tile's pages, -1: no page (for the softmax warps, for the V warps)
+    int* const s_info = reinterpret_cast<int*>(s_nan + R * (DH / 32));
+    uint64_t* const bars = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(s_info + 2 * C::INFO * TCA_PAGES) + 7) & ~uintptr_t(7));
+    Seg* const segs = reinterpret_cast<Seg*>(bars + 64);
+    Seg* const s_cut = segs + A8_SEGS;  // [2]
+    unsigned* const s_scan = reinterpret_cast<unsigned*>(s_cut + 2);
+    int* const s_last = reinterpret_cast<int*>(s_scan + A8_SCAN);  // [2]
+    int* const s_flag = s_last + 2;                                 // NaN cells seen
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(s_flag + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rep = p.H / p.G;
+    // barriers
+    const uint32_t b0 = smem_u32(bars);
+    const uint32_t k_full = b0, k_empty = k_full + 8 * NK, v_full = k_empty + 8 * NK, v_empty = v_full + 8 * NV;
+    const uint32_t s_full = v_empty + 8 * NV, s_empty = s_full + 16, p_full = s_empty + 16, p_empty = p_full + 16;
+    const uint32_t w_full = p_empty + 16, w_empty = w_full + 8 * NV16;  // f16 V
+    const uint32_t q_full = w_empty + 8 * NV16, q_empty = q_full + 16, o_full = q_empty + 16, o_empty = o_full + 16;
+    const uint32_t l_full = o_empty + 16, l_empty = l_full + 16;
+    static_assert(2 * NK + 2 * NV + 2 * NV16 + 18 <= 64, "barriers");
+    if (threadIdx.x == 0) {
+        const auto init = [](uint32_t bar, int n, int count) {
+            for (int i = 0; i < n; ++i) mbar_init(bar + 8 * i, (uint32_t)count);
+        };
+        init(k_full, NK, 1);
+        init(k_empty, NK, 1);
+        init(v_full, NV, 1);
+        init(v_empty, NV, 4);
+        init(s_full, 2, 2);   // the products, and the MMA thread itself (it passes on what it has seen)
+        init(s_empty, 2, 8);
+        init(p_full, 2, 8);
+        init(p_empty, 2, 1);
+        init(w_full, NV16, 4);
+        init(w_empty, NV16, 1);
+        init(q_full, 2, 1);
+        init(q_empty, 2, 9);  // the products, and the softmax warps (score factors)
+        init(o_full, 2, 1);
+        init(o_empty, 2, 4);
+        init(l_full, 2, 8);
+        init(l_empty, 2, 4);
+        mbar_fence_init();
+        *s_flag = s_last[0] = s_last[1] = 0;
+    }
+    for (int i = threadIdx.x; i < R * (DH / 32); i += TCA_THREADS) s_nan[i] = 0;
+    pdl_wait();
+    A8Work work;
+    const bool busy = a8_plan<TCA_THREADS, TCA_PAGES>(p, R, rep, s_scan, work);  // (block-uniform)
+    if (!busy) return;
+    if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
+    a8_list<TCA_PAGES>(p, R, rep, work, 0, segs);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_trigger();  // (after the TMEM is taken: a kernel that starts early does not take it first)
+    const uint32_t tmem = *s_tmem;
+    const auto col_s = [&](int b) { return tmem + (uint32_t)(b * C::S_COLS); };
+    const auto col_o = [&](int b) { return tmem + (uint32_t)(2 * C::S_COLS + b * C::O_COLS); };
+
+    // per role, through all rounds
+    bool dead = false;  // a bounded wait ran out: the role goes through the motions without touching memory
+    const auto wait = [&](uint32_t bar, int parity) {
+        if (!dead && !mbar_try_wait(bar, (uint32_t)parity)) dead = !wait_longer(bar, (uint32_t)parity, p.err);
+    };
+    Turn<NK> kt;
+    Turn<NV> vt;
+    Turn<2> st, pt, qt, ot;
+    Turn<NV16> wt;
+    int tile = 0;           // of this CTA (page words)
+
+    for (int seg0 = 0; seg0 < work.nspans; seg0 += A8_SEGS) {
+        if (seg0 > 0) {
+            __syncwarp();
+            __syncthreads();
+            a8_list<TCA_PAGES>(p, R, rep, work, seg0, segs);
+            __syncthreads();
+        }
+        const int nseg = min(A8_SEGS, work.nspans - seg0);
+        if (warp < 8) {
+            // ---------------- softmax: key 32 * quad + lane of each tile, rows r0 .. r0 + RH - 1 ----------------
+            constexpr int RH = C::RH, BATCH = RH > 16 ? RH / 2 : RH;  // rows read from TMEM at a time
+            const int quad = warp & 3, r0 = (warp >> 2) * RH, key = 32 * quad + lane;
+            const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+            // this key's weights in P, [key][row], 16-byte chunks swizzled by the key
+            const uint32_t p_sw = (uint32_t)(C::PROW == 128 ? key & 7 : C::PROW == 64 ? key >> 1 & 3 : key >> 2 & 1) << 4;
+            const uint32_t p_at = smem_u32(s_p) + (uint32_t)(key * C::PROW);
+#pragma unroll 1
+            for (int si = 0; si < nseg; ++si) {
+                const Seg sg = segs[si];
+                const int rows = sg.rows, pos_last = sg.pos + div_rep(p, sg.rem + rows - 1);
+                if (threadIdx.x < R) {
+                    const int n = threadIdx.x;
+                    s_neg[n] = 0.f;
+                    s_set[n] = 0;
+                    s_pos[n] = n < rows ? sg.pos + div_rep(p, sg.rem + n) : -0x40000000;  // (no key is seen)
+                }
+                softmax_bar();
+                const unsigned w = p.window > 0 ? (unsigned)p.window : 0x80000000u;
+                bool force = true;  // some row has not seen a key yet
+                float2 l[RH / 2];
+#pragma unroll
+                for (int n = 0; n < RH / 2; ++n) l[n] = make_float2(0.f, 0.f);
+#pragma unroll 1
+                for (int i = 0; i < sg.n; ++i, ++tile) {
+                    const int j0 = (sg.page + TCA_PAGES * i) * 16;
+                    wait(s_full + 8 * st.slot, st.phase);
+                    tc_fence_after();
+                    const int info = s_info[(tile & (C::INFO - 1)) * TCA_PAGES + 2 * quad + (lane >> 4)];
+                    const bool here = info >= 0;
+                    const int ek = here ? (info & 255) - 128 : 0, ev = here ? (info >> 8) - 128 : 0;
+                    const float fk = exp2_int(ek), inv = exp2_int(-ev);
+                    const float2 fk2 = make_float2(fk, fk), shift = make_float2((float)ev, (float)ev), inv2 = make_float2(inv, inv);
+                    const bool plain = p.cap <= 0.f && all_seen(p, sg, pos_last, j0) && __all_sync(0xffffffffu, here);
+                    const float* const rf = s_rf + qt.slot * R + r0;
+                    const uint32_t at = col_s(st.slot) + lanes + (uint32_t)r0;
+                    float2 d[RH / 2];  // score + e_V - reference, rows r0 + 2 n, + 1
+#pragma unroll
+                    for (int b0 = 0; b0 < RH; b0 += BATCH) {
+                        uint32_t x[BATCH], y[BATCH];
+                        tmem_ld<BATCH>(at + (uint32_t)b0, x);
+                        tmem_ld<BATCH>(at + (uint32_t)(R + b0), y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int n = 0; n < BATCH; n += 2)
+                            d[(b0 + n) / 2] = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f),
+                                                   make_float2(__uint_as_float(x[n]), __uint_as_float(x[n + 1])));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * st.slot);
+                    st.next();
+#pragma unroll
+                    for (int n = 0; n < RH; n += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(rf + n), m = *reinterpret_cast<const float4*>(s_neg + r0 + n);
+                        float2 a = mul2(d[n / 2], fk2), b = mul2(d[n / 2 + 1], fk2);
+                        const float2 ma = add2(shift, make_float2(m.x, m.y)), mb = add2(shift, make_float2(m.z, m.w));
+                        if (p.cap > 0.f) {
+                            a = add2(make_float2(cap_score(p, a.x * f.x), cap_score(p, a.y * f.y)), ma);
+                            b = add2(make_float2(cap_score(p, b.x * f.z), cap_score(p, b.y * f.w)), mb);
+                        } else {
+                            a = fma2(a, make_float2(f.x, f.y), ma);
+                            b = fma2(b, make_float2(f.z, f.w), mb);
+                        }
+                        d[n / 2] = a;
+                        d[n / 2 + 1] = b;
+                    }
+                    if (!plain) {
+                        const int kj = j0 + key;
+                        const unsigned wk = here ? w : 0u;
+#pragma unroll
+                        for (int n = 0; n < RH; n += 4) {
+                            const int4 q = *reinterpret_cast<const int4*>(s_pos + r0 + n);
+                            float2 &a = d[n / 2], &b = d[n / 2 + 1];
+                            a.x = (unsigned)(q.x - kj) < wk ? a.x : -INFINITY;
+                            a.y = (unsigned)(q.y - kj) < wk ? a.y : -INFINITY;
+                            b.x = (unsigned)(q.z - kj) < wk ? b.x : -INFINITY;
+                            b.y = (unsigned)(q.w - kj) < wk ? b.y : -INFINITY;
+                        }
+                    }
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < RH / 2; ++n) top = fmaxf(top, fmaxf(d[n].x, d[n].y));
+                    // move the references: at a row's first keys, and before a weight would pass 2^15
+                    if (softmax_or(force || top > 15.f)) {
+#pragma unroll
+                        for (int n = 0; n < RH; ++n) {
+                            const float x = warp_fmax(n & 1 ? d[n / 2].y : d[n / 2].x);
+                            if (lane == n) s_mx[quad * R + r0 + n] = x;
+                        }
+                        softmax_bar();
+                        bool unset = false;
+                        if (threadIdx.x < R) {
+                            const int n = threadIdx.x;
+                            const float x = fmaxf(fmaxf(s_mx[n], s_mx[R + n]), fmaxf(s_mx[2 * R + n], s_mx[3 * R + n]));
+                            const float was = -s_neg[n];
+                            const bool set = s_set[n] != 0;
+                            const float now = x == -INFINITY ? was : set ? fmaxf(was, was + (x - 7.f)) : was + (x - 7.f);
+                            s_f[n] = set ? ex2(was - now) : 1.f;
+                            s_dm[n] = was - now;
+                            s_neg[n] = -now;
+                            if (x > -INFINITY) s_set[n] = 1;
+                            unset = n < rows && !set && x == -INFINITY;
+                        }
+                        force = softmax_or(unset);
+#pragma unroll
+                        for (int n = 0; n < RH; n += 4) {
+                            const float4 a = *reinterpret_cast<const float4*>(s_dm + r0 + n), f = *reinterpret_cast<const float4*>(s_f + r0 + n);
+                            d[n / 2] = add2(d[n / 2], make_float2(a.x, a.y));
+                            d[n / 2 + 1] = add2(d[n / 2 + 1], make_float2(a.z, a.w));
+                            l[n / 2] = mul2(l[n / 2], make_float2(f.x, f.y));
+                            l[n / 2 + 1] = mul2(l[n / 2 + 1], make_float2(f.z, f.w));
+                        }
+                        if (i > 0) {
+                            // O^T follows, once the products of the tile before are done
+                            wait(p_empty + 8 * (pt.slot ^ 1), pt.slot ? pt.phase : pt.phase ^ 1);
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int n = 0; n < C::HALVES * RH; n += 4) {
+                                const int n0 = r0 + n % RH;
+                                const uint32_t o_at = col_o(ot.slot) + lanes + (uint32_t)((n / RH) * RP + n0);
+                                uint32_t x[4];
+                                tmem_ld<4>(o_at, x);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int z = 0; z < 4; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * s_f[n0 + z]);
+                                tmem_st4(o_at, x);
+                            }
+                            tmem_wait_st();
+                            tc_fence_before();
+                        }
+                    }
+                    // weights
+                    wait(p_empty + 8 * pt.slot, pt.phase ^ 1);
+                    const uint32_t pa = p_at + (uint32_t)(pt.slot * C::PB);
+                    if (!dead) {
+                        constexpr int PER = RH % 8 == 0 ? 8 : 4;  // rows a store
+#pragma unroll
+                        for (int n = 0; n < RH; n += PER) {
+                            uint32_t h[PER / 2];
+#pragma unroll
+                            for (int z = 0; z < PER / 2; ++z) {
+                                const float2 x = make_float2(ex2(d[n / 2 + z].x), ex2(d[n / 2 + z].y));
+                                l[n / 2 + z] = fma2(x, inv2, l[n / 2 + z]);
+                                h[z] = f16x2_of(x.x, x.y);
+                            }
+                            const uint32_t at_row = (uint32_t)(r0 + n) * 2;
+                            const uint32_t a = pa + ((at_row & ~15u) ^ p_sw) + (at_row & 8u);
+                            if constexpr (PER == 8) sts128(a, h[0], h[1], h[2], h[3]);
+                            else sts64(a, h[0], h[1]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 8 * pt.slot);
+                    pt.next();
+                }
+                // the span's sums over the warp's keys, and its references, for the warps that write the result
+                wait(l_empty + 8 * ot.slot, ot.phase ^ 1);
+                float* const lt = s_lt + warp * 4 * C::LDL;
+#pragma unroll
+                for (int n = 0; n < RH; n += 4) {
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) lt[z * C::LDL + lane] = z & 1 ? l[(n + z) / 2].y : l[(n + z) / 2].x;
+                    __syncwarp();
+                    const float* const at = lt + (lane >> 3) * C::LDL + (lane & 7) * 4;
+                    float x = (at[0] + at[1]) + (at[2] + at[3]);
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    if ((lane & 7) == 0) s_l[(ot.slot * 4 + quad) * R + r0 + n + (lane >> 3)] = x;
+                    __syncwarp();
+                }
+                if (threadIdx.x < R) s_mo[ot.slot * R + threadIdx.x] = -s_neg[threadIdx.x];
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(l_full + 8 * ot.slot);
+                    mbar_arrive(q_empty + 8 * qt.slot);
+                }
+                qt.next();
+                ot.next();
+                softmax_bar();  // (s_neg has been read)
+            }
+        } else if (warp < 12) {
+            // ---------------- V: e4m3 -> f16, and the results ----------------
+            const int tid = threadIdx.x - 256, quad = warp & 3;
+            constexpr int C16 = DH / 16, KEYS = 128 / C16;  // 16-byte pieces of a key; keys the warps take at a time
+            const int c16 = tid % C16, key0 = tid / C16;
+            const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+            // places of a piece's two 16-byte chunks in a 128-byte row of f16, by key & 7 (swizzle); lanes of one
+            // 64-dim block store them in the other order (bank conflicts)
+            const int sw = (c16 >> 2) & 1;
+            const uint32_t chunk = (uint32_t)(((2 * c16) & 7) << 4);
+#pragma unroll 1
+            for (int si = 0; si < nseg; ++si) {
+                const Seg sg = segs[si];
+                const int rows = sg.rows, pos_last = sg.pos + div_rep(p, sg.rem + rows - 1);
+#pragma unroll 1
+                for (int i = 0; i < sg.n; ++i, ++tile) {
+                    const int j0 = (sg.page + TCA_PAGES * i) * 16;
+                    wait(v_full + 8 * vt.slot, vt.phase);
+                    wait(w_empty + 8 * wt.slot, wt.phase ^ 1);
+                    const int* const info = s_info + C::INFO * TCA_PAGES + (tile & (C::INFO - 1)) * TCA_PAGES;
+                    const int4 i0 = *reinterpret_cast<const int4*>(info), i1 = *reinterpret_cast<const int4*>(info + 4);
+                    const bool plain = all_seen(p, sg, pos_last, j0) && (i0.x | i0.y | i0.z | i0.w | i1.x | i1.y | i1.z | i1.w) >= 0;
+                    const uint32_t src = smem_u32(v_ring + vt.slot * C::KT) + (uint32_t)(tid * 16);
+                    const uint32_t dst = smem_u32(v16 + wt.slot * C::V16) + (uint32_t)((c16 >> 2) * 16384);
+                    if (!dead && !plain) {
+                        // cells without a page hold whatever the ring held: zeros instead.  A NaN cell must reach
+                        // the rows that see its key and no others: it is taken out of the product, and noted for
+                        // the rows it belongs to
+#pragma unroll 1
+                        for (int it = 0; it < 128 / KEYS; ++it) {
+                            const int key = it * KEYS + key0;
+                            const uint32_t at = src + (uint32_t)(it * 2048);
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+                            if (info[key >> 4] < 0) w[0] = w[1] = w[2] = w[3] = 0;
+                            uint32_t any = 0;
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) {
+                                const uint32_t bad = ((w[z] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                                w[z] &= ~(bad | (bad - (bad >> 7)));
+                                any |= bad;
+                            }
+                            if (any)
+                                note_nans(at, c16 * 16, j0 + key, sg.pos, sg.rem, p.rep_magic, rows, p.window, DH / 32, s_nan, s_flag);
+                            sts128(at, w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    if (!dead) {
+                        // 8 bytes to one 16-byte chunk, twice: lanes of one 64-dim block take their two chunks in the
+                        // other order (bank conflicts)
+                        const uint32_t from = src + (uint32_t)(sw * 8), to = dst + (chunk ^ (uint32_t)(sw << 4));
+#pragma unroll 4
+                        for (int it = 0; it < 128 / KEYS; ++it) {
+                            const int key = it * KEYS + key0;
+                            const uint32_t at = from + (uint32_t)(it * 2048);
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+                            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(at ^ 8u));
+                            const uint32_t a = (to ^ (uint32_t)((key & 7) << 4)) + (uint32_t)((key >> 3) * 1024 + (key & 7) * 128);
+                            sts128(a, f16x2_lo(w[0]), f16x2_hi(w[0]), f16x2_lo(w[1]), f16x2_hi(w[1]));
+                            sts128(a ^ 16u, f16x2_lo(w[2]), f16x2_hi(w[2]), f16x2_lo(w[3]), f16x2_hi(w[3]));
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(v_empty + 8 * vt.slot);
+                        mbar_arrive(w_full + 8 * wt.slot);
+                    }
+                    vt.next();
+                    wt.next();
+                }
+                // ---- the span's result: this thread's dim is 32 * quad + lane of each half
+                const bool whole = sg.c0 == sg.c1;
+                wait(l_full + 8 * ot.slot, ot.phase);
+                if (tid < rows) {
+                    const float* const lp = s_l + ot.slot * 4 * R + tid;
+                    const float L = (lp[0] + lp[R]) + (lp[2 * R] + lp[3 * R]);
+                    const long long part_row = (long long)(2 * blockIdx.x + ((int)blockIdx.x == sg.c0 ? 1 : 0)) * R + tid;
+                    const int tok = div_rep(p, sg.rem + tid);
+                    s_inv[tid] = !whole ? 1.f : L == 0.f ? 0.f : 1.0f / L;
+                    s_off[tid] = whole ? (long long)(sg.tok + tok) * p.out_stride + (long long)(sg.g * rep + sg.rem + tid - tok * rep) * DH
+                                       : part_row * DH;
+                    if (!whole) __stcg(p.ws_ml + part_row, make_float2(L == 0.f ? A8_LOWEST : s_mo[ot.slot * R + tid], L));
+                }
+                v_bar();
+                const bool nans = *s_flag != 0;
+                wait(o_full + 8 * ot.slot, ot.phase);
+                tc_fence_after();
+#pragma unroll 1
+                for (int half = 0; half < C::HALVES; ++half) {
+                    const int dim = half * 128 + 32 * quad + lane;
+#pragma unroll 1
+                    for (int n0 = 0; n0 < rows; n0 += 8) {
+                        uint32_t x[8];
+                        tmem_ld<8>(col_o(ot.slot) + lanes + (uint32_t)(half * RP + n0), x);
+                        tmem_wait_ld();
+                        if (dim >= DH || dead) continue;
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) {
+                            if (n0 + z < rows) {
+                                float v = __uint_as_float(x[z]) * s_inv[n0 + z];
+                                if (nans && (s_nan[(n0 + z) * (DH / 32) + (dim >> 5)] >> (dim & 31) & 1)) v = __int_as_float(0x7fffffff);
+                                if (whole) reinterpret_cast<__nv_bfloat16*>(p.out)[s_off[n0 + z] + dim] = __float2bfloat16_rn(v);
+                                else __stcg(p.ws_o + s_off[n0 + z] + dim, v);
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+                v_bar();  // (a cut span's part is written; s_inv, s_off and the NaN notes have been read)
+                if (nans) {
+                    for (int z = tid; z < R * (DH / 32); z += 128) s_nan[z] = 0;
+                    if (tid == 0) *s_flag = 0;
+                    v_bar();
+                }
+                if (lane == 0) {
+                    mbar_arrive(o_empty + 8 * ot.slot);
+                    mbar_arrive(l_empty + 8 * ot.slot);
+                }
+                ot.next();
+                if (!whole && tid == 0) a8_arrive(p, sg, s_last, s_cut);
+            }
+        } else if (warp < 14) {
+            // ---------------- copies: K (warp 12) and V (warp 13) ----------------
+            // lane: page lane & 7 of tile lane / 8 of a batch of four tiles of one span
+            const bool is_v = warp == 13;
+            int* const info = s_info + (is_v ? C::INFO * TCA_PAGES : 0);
+            // (block ids are asked for two batches ahead, scale bytes one: nobody waits for either)
+            int id = -1, id2 = -1, id3 = -1, g3 = 0;
+            bool has3 = false;
+            uint32_t kb = 0, vb = 0, kb2 = 0, vb2 = 0;
+            int fsi = 0, fi = 0;  // the batch to ask for next
+            const auto ids = [&]() {
+                has3 = false;
+                if (fsi >= nseg) return;
+                const Seg& sg = segs[fsi];
+                const int page = sg.page + TCA_PAGES * fi + lane;
+                has3 = fi + (lane >> 3) < sg.n && page < sg.pend;
+                g3 = sg.g;
+                if (has3) id3 = p.tables[(size_t)sg.b * p.max_blocks + page];
+                fi += 4;
+                if (fi >= sg.n) {
+                    fi = 0;
+                    ++fsi;
+                }
+            };
+            const auto scales = [&]() {
+                id2 = -1;
+                if (!has3) return;
+                if (id3 < 0 || id3 >= p.num_blocks) {
+                    raise_err(p.err, YK_DEV_ERR_BOUNDS);
+                    return;
+                }
+                id2 = id3;
+                if (!is_v) {
+                    const uint8_t* const s = p.scales + (size_t)id3 * p.block_scales + p.layer_scale + g3;
+                    kb2 = s[0];
+                    vb2 = s[p.G];
+                }
+            };
+            ids();
+            scales();
+            ids();
+#pragma unroll 1
+            for (int si = 0; si < nseg; ++si) {
+                const int n = segs[si].n, g = segs[si].g;
+#pragma unroll 1
+                for (int i = 0; i < n; ++i, ++tile) {
+                    if ((i & 3) == 0) {
+                        id = id2;
+                        kb = kb2;
+                        vb = vb2;
+                        scales();
+                        ids();
+                    }
+                    const bool mine = lane >> 3 == (i & 3);  // this lane's page belongs to the tile
+                    const int pages = __popc(__ballot_sync(0xffffffffu, mine && id >= 0));
+                    const uint32_t bar = is_v ? v_full + 8 * vt.slot : k_full + 8 * kt.slot;
+                    wait(is_v ? v_empty + 8 * vt.slot : k_empty + 8 * kt.slot, (is_v ? vt.phase : kt.phase) ^ 1);
+                    dead = __any_sync(0xffffffffu, dead);
+                    if (mine)
+                        info[(tile & (C::INFO - 1)) * TCA_PAGES + (lane & 7)] =
+                            id < 0 ? -1 : (kv8_exponent(kb) + 128) | (kv8_exponent(vb) + 128) << 8;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_expect_tx(bar, dead ? 0u : (uint32_t)(pages * 16 * DH));
+                    __syncwarp();
+                    if (mine && id >= 0 && !dead) {
+                        if (is_v) {
+                            bulk_load(smem_u32(v_ring + vt.slot * C::KT) + (uint32_t)((lane & 7) * 16 * DH),
+                                      p.pool + (size_t)id * p.block_cells + p.layer_off + (size_t)(p.G + g) * 16 * DH, 16 * DH, bar);
+                        } else {
+                            const uint32_t dst = smem_u32(k_ring + kt.slot * C::KT) + (uint32_t)((lane & 7) * 16 * C::ROWB);
+#pragma unroll
+                            for (int x = 0; x < C::BOXES; ++x)
+                                asm volatile(
+                                    "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+                                    " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst + (uint32_t)(x * TCA_TILE * 128)),
+                                    "l"((uint64_t)&map), "r"(x * 128), "r"(g * 16), "r"(0), "r"(p.layer), "r"(id), "r"(bar)
+                                    : "memory");
+                        }
+                    }
+                    if (is_v) vt.next();
+                    else kt.next();
+                }
+            }
+        } else if (warp == 14) {
+            // ---------------- MMA: one thread ----------------
+            if (lane == 0) {
+                // f32 accumulators; S^T: e4m3 both; O^T: f16 both, A (V) with its M side contiguous
+                constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::S_COLS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+                constexpr uint32_t idesc_o = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(RP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+                constexpr uint32_t hi_s = desc_hi(8 * C::ROWB, DH == 64 ? 4 : 2), hi_v = desc_hi(1024, 2);
+                constexpr uint32_t hi_p = desc_hi(8 * C::PROW, C::PROW == 128 ? 2 : C::PROW == 64 ? 4 : 6);
+                constexpr uint32_t v_lbo = DH == 64 ? 0 : 16384;  // (64 dims: the product's other 64 rows repeat them)
+                // O^T of tile (pending): its span's buffer and whether it begins or ends the span
+                bool pending = false, begins = false, ends = false;
+                const auto values = [&]() {
+                    if (begins) wait(o_empty + 8 * ot.slot, ot.phase ^ 1);
+                    wait(p_full + 8 * pt.slot, pt.phase);
+                    wait(w_full + 8 * wt.slot, wt.phase);
+                    tc_fence_after();
+                    if (!dead) {
+                        const uint32_t va = desc_lo(smem_u32(v16 + wt.slot * C::V16), v_lbo), pa = desc_lo(smem_u32(s_p + pt.slot * C::PB));
+                        const uint32_t d = col_o(ot.slot);
+#pragma unroll
+                        for (int half = 0; half < C::HALVES; ++half)
+#pragma unroll
+                            for (int ks = 0; ks < 8; ++ks)
+                                mma_tc<false>(d + (uint32_t)(half * RP), va + (uint32_t)(half * 2048 + ks * 128), hi_v,
+                                              pa + (uint32_t)(ks * C::PROW), hi_p, idesc_o, begins && ks == 0 ? 0u : 1u);
+                        tc_commit(p_empty + 8 * pt.slot);
+                        tc_commit(w_empty + 8 * wt.slot);
+                        if (ends) tc_commit(o_full + 8 * ot.slot);
+                    }
+                    pt.next();
+                    wt.next();
+                    if (ends) ot.next();
+                    pending = false;
+                };
+#pragma unroll 1
+                for (int si = 0; si < nseg; ++si) {
+                    const int n = segs[si].n;
+                    wait(q_full + 8 * qt.slot, qt.phase);
+#pragma unroll 1
+                    for (int i = 0; i < n; ++i) {
+                        wait(k_full + 8 * kt.slot, kt.phase);
+                        wait(s_empty + 8 * st.slot, st.phase ^ 1);
+                        tc_fence_after();
+                        if (!dead) {
+                            const uint32_t ka = desc_lo(smem_u32(k_ring + kt.slot * C::KT)), qa = desc_lo(smem_u32(s_q + qt.slot * C::QB));
+                            const uint32_t d = col_s(st.slot);
+#pragma unroll
+                            for (int ks = 0; ks < DH / 32; ++ks)
+                                mma_tc<true>(d, ka + (uint32_t)((ks >> 2) * (TCA_TILE * 8) + (ks & 3) * 2), hi_s,
+                                             qa + (uint32_t)((ks >> 2) * (2 * R * 8) + (ks & 3) * 2), hi_s, idesc_s, ks == 0 ? 0u : 1u);
+                            tc_commit(k_empty + 8 * kt.slot);
+                            tc_commit(s_full + 8 * st.slot);
+                            if (i == n - 1) tc_commit(q_empty + 8 * qt.slot);
+                        }
+                        mbar_arrive(s_full + 8 * st.slot);
+                        kt.next();
+                        st.next();
+                        if (pending) values();
+                        pending = true;
+                        begins = i == 0;
+                        ends = i == n - 1;
+                    }
+                    qt.next();
+                }
+                if (pending) values();
+            }
+        } else {
+            // ---------------- queries: two e4m3 terms of each row ----------------
+            constexpr int LPR = DH / 16, RPI = 32 / LPR;  // lanes a row, rows at a time
+            const int c16 = lane % LPR;
+#pragma unroll 1
+            for (int si = 0; si < nseg; ++si) {
+                const Seg& sg = segs[si];
+                uint4 x[2], y[2];  // 16 values; the next rows' come while these convert
+                const auto load = [&](int r0, uint4 (&v)[2]) {
+                    const int row = r0 + lane / LPR;
+                    v[0] = v[1] = make_uint4(0, 0, 0, 0);
+                    if (row < sg.rows) {
+                        const int tok = div_rep(p, sg.rem + row);
+                        const uint4* const src = reinterpret_cast<const uint4*>(
+                            reinterpret_cast<const __nv_bfloat16*>(p.q) + (size_t)(sg.tok + tok) * p.q_stride +
+                            (size_t)(sg.g * rep + sg.rem + row - tok * rep) * DH + c16 * 16);
+                        v[0] = __ldcg(src);
+                        v[1] = __ldcg(src + 1);
+                    }
+                };
+                load(0, x);
+                wait(q_empty + 8 * qt.slot, qt.phase ^ 1);
+#pragma unroll 1
+                for (int r0 = 0; r0 < R; r0 += RPI) {
+                    load(r0 + RPI, y);
+                    const int row = r0 + lane / LPR;
+                    float f[16];
+                    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+                    float amax = 0.f;
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) {
+                        f[2 * z] = __uint_as_float(w[z] << 16);
+                        f[2 * z + 1] = __uint_as_float(w[z] & 0xffff0000u);
+                        amax = fmaxf(amax, fmaxf(fabsf(f[2 * z]), fabsf(f[2 * z + 1])));
+                    }
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    // 2^-e brings the row's largest value to at most 448
+                    const uint32_t bits = __float_as_uint(amax);
+                    const int e = amax == 0.f ? 0 : max(-100, min(100, (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0)));
+                    const float g = exp2_int(-e);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        hi[z] = lo[z] = 0;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float a = f[4 * z + 2 * k] * g, b = f[4 * z + 2 * k + 1] * g;
+                            const uint32_t h = e4m3x2_from(a, b);
+                            const float2 back = f32x2(f16x2_lo(h));
+                            hi[z] |= h << (16 * k);
+                            lo[z] |= e4m3x2_from((a - back.x) * 16.f, (b - back.y) * 16.f) << (16 * k);
+                        }
+                    }
+                    if (row < R && !dead) {
+                        if (c16 == 0) s_rf[qt.slot * R + row] = p.scale_log2 * exp2_int(e);
+                        // [128-dim block][row][128 bytes] (DH 64: 64 bytes), swizzled; second terms are rows R ..
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int n = row + t * R;
+                            const uint32_t at = DH == 64 ? (uint32_t)(n * 64 + ((c16 ^ ((n >> 1) & 3)) << 4))
+                                                         : (uint32_t)((c16 >> 3) * (2 * R * 128) + n * 128 + (((c16 & 7) ^ (n & 7)) << 4));
+                            const uint32_t* const v = t ? lo : hi;
+                            sts128(smem_u32(s_q + qt.slot * C::QB) + at, v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                    x[0] = y[0];
+                    x[1] = y[1];
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full + 8 * qt.slot);
+                qt.next();
+            }
+        }
+    }
+    // every copy asked for has landed before the CTA ends (its readers waited for it, unless they gave up)
+    if (dead && (warp == 12 || warp == 13) && lane == 0)
+        for (int i = 0; i < (warp == 12 ? NK : NV); ++i)
+            for (int ph = 0; ph < 2; ++ph)
+                (void)mbar_wait_bounded_ns((warp == 12 ? k_full : v_full) + 8 * i, (uint32_t)ph, 100000000ull);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 14) tmem_dealloc(tmem, C::TMEM);
+    a8_join<__nv_bfloat16, DH, TCA_THREADS>(p, R, rep, s_last, s_cut);
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+template <int DH, int RN>
+static yk_status launch_tca(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, const Attn8Params& p) {
+    using C = TcaCfg<DH, RN>;
+    static_assert(C::R <= A8_WS / DH, "cut spans' rows in the workspace");
+    int dev = 0;
+    YK_CHECK_CUDA(cudaGetDevice(&dev));
+    static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(ready.load(std::memory_order_acquire) & bit)) {
+        YK_CHECK_CUDA(cudaFuncSetAttribute(attn8_tc_kernel<DH, RN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        ready.fetch_or(bit, std::memory_order_release);
+    }
+    YK_CHECK_CUDA(launch_on(st, pdl, attn8_tc_kernel<DH, RN>, num_sms, TCA_THREADS, C::SMEM, map, p));
+    return YK_OK;
+}
+
+// rows: (token, head) rows of a sequence's new tokens, as far as the caller says.
+// The tile holds them all up to 64 (head_dim 256: 16), rounded up to the next shape.
+template <int DH>
+static yk_status launch_tca_rows(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, const Attn8Params& p,
+                                 long long rows) {
+    if (rows <= 8) return launch_tca<DH, 1>(st, pdl, num_sms, map, p);
+    if (DH == 256 || rows <= 16) return launch_tca<DH, 2>(st, pdl, num_sms, map, p);
+    if constexpr (DH != 256) {
+        if (rows <= 24) return launch_tca<DH, 3>(st, pdl, num_sms, map, p);
+        if (rows <= 32) return launch_tca<DH, 4>(st, pdl, num_sms, map, p);
+        if (rows <= 48) return launch_tca<DH, 6>(st, pdl, num_sms, map, p);
+        return launch_tca<DH, 8>(st, pdl, num_sms, map, p);
+    }
+    return YK_OK;
+}
+
+yk_status attention_e4m3_launch_bf16(cudaStream_t st, bool pdl, int num_sms, int head_dim, const CUtensorMap& map,
+                                     const Attn8Params& p, long long rows) {
+    switch (head_dim) {
+        case 64: return launch_tca_rows<64>(st, pdl, num_sms, map, p, rows);
+        case 128: return launch_tca_rows<128>(st, pdl, num_sms, map, p, rows);
+        default: return launch_tca_rows<256>(st, pdl, num_sms, map, p, rows);
+    }
+}
+
+}  // namespace yk
