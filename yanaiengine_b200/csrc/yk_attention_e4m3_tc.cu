@@ -189,6 +189,12 @@ __device__ __noinline__ void note_nans(uint32_t cells, int dim0, int key, int po
     }
 }
 
+__device__ __forceinline__ bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // A ring's next place: slot and the parity of its use.
 template <int N>
 struct Turn {
@@ -361,20 +367,20 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_empty + 8 * st.slot);
                     st.next();
+                    if (p.cap <= 0.f) {
 #pragma unroll
-                    for (int n = 0; n < RH; n += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(rf + n), m = *reinterpret_cast<const float4*>(s_neg + r0 + n);
-                        float2 a = mul2(d[n / 2], fk2), b = mul2(d[n / 2 + 1], fk2);
-                        const float2 ma = add2(shift, make_float2(m.x, m.y)), mb = add2(shift, make_float2(m.z, m.w));
-                        if (p.cap > 0.f) {
-                            a = add2(make_float2(cap_score(p, a.x * f.x), cap_score(p, a.y * f.y)), ma);
-                            b = add2(make_float2(cap_score(p, b.x * f.z), cap_score(p, b.y * f.w)), mb);
-                        } else {
-                            a = fma2(a, make_float2(f.x, f.y), ma);
-                            b = fma2(b, make_float2(f.z, f.w), mb);
+                        for (int n = 0; n < RH; n += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(rf + n), m = *reinterpret_cast<const float4*>(s_neg + r0 + n);
+                            d[n / 2] = fma2(mul2(d[n / 2], fk2), make_float2(f.x, f.y), add2(shift, make_float2(m.x, m.y)));
+                            d[n / 2 + 1] = fma2(mul2(d[n / 2 + 1], fk2), make_float2(f.z, f.w), add2(shift, make_float2(m.z, m.w)));
                         }
-                        d[n / 2] = a;
-                        d[n / 2 + 1] = b;
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < RH; n += 2) {
+                            const float2 f = *reinterpret_cast<const float2*>(rf + n), m = *reinterpret_cast<const float2*>(s_neg + r0 + n);
+                            const float2 x = mul2(mul2(d[n / 2], fk2), f);
+                            d[n / 2] = add2(make_float2(cap_score(p, x.x), cap_score(p, x.y)), add2(shift, m));
+                        }
                     }
                     if (!plain) {
                         const int kj = j0 + key;
@@ -671,11 +677,10 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     const bool mine = lane >> 3 == (i & 3);  // this lane's page belongs to the tile
                     const int pages = __popc(__ballot_sync(0xffffffffu, mine && id >= 0));
                     const uint32_t bar = is_v ? v_full + 8 * vt.slot : k_full + 8 * kt.slot;
-                    wait(is_v ? v_empty + 8 * vt.slot : k_empty + 8 * kt.slot, (is_v ? vt.phase : kt.phase) ^ 1);
-                    dead = __any_sync(0xffffffffu, dead);
                     if (mine)
                         info[(tile & (C::INFO - 1)) * TCA_PAGES + (lane & 7)] =
                             id < 0 ? -1 : (kv8_exponent(kb) + 128) | (kv8_exponent(vb) + 128) << 8;
+                    wait(is_v ? v_empty + 8 * vt.slot : k_empty + 8 * kt.slot, (is_v ? vt.phase : kt.phase) ^ 1);
                     __syncwarp();
                     if (lane == 0) mbar_arrive_expect_tx(bar, dead ? 0u : (uint32_t)(pages * 16 * DH));
                     __syncwarp();
@@ -699,71 +704,72 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                 }
             }
         } else if (warp == 14) {
-            // ---------------- MMA: one thread ----------------
-            if (lane == 0) {
-                // f32 accumulators; S^T: e4m3 both; O^T: f16 both, A (V) with its M side contiguous
-                constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::S_COLS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-                constexpr uint32_t idesc_o = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(RP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-                constexpr uint32_t hi_s = desc_hi(8 * C::ROWB, DH == 64 ? 4 : 2), hi_v = desc_hi(1024, 2);
-                constexpr uint32_t hi_p = desc_hi(8 * C::PROW, C::PROW == 128 ? 2 : C::PROW == 64 ? 4 : 6);
-                constexpr uint32_t v_lbo = DH == 64 ? 0 : 16384;  // (64 dims: the product's other 64 rows repeat them)
-                // O^T of tile (pending): its span's buffer and whether it begins or ends the span
-                bool pending = false, begins = false, ends = false;
-                const auto values = [&]() {
-                    if (begins) wait(o_empty + 8 * ot.slot, ot.phase ^ 1);
-                    wait(p_full + 8 * pt.slot, pt.phase);
-                    wait(w_full + 8 * wt.slot, wt.phase);
-                    tc_fence_after();
-                    if (!dead) {
-                        const uint32_t va = desc_lo(smem_u32(v16 + wt.slot * C::V16), v_lbo), pa = desc_lo(smem_u32(s_p + pt.slot * C::PB));
-                        const uint32_t d = col_o(ot.slot);
+            // ---------------- MMA: the warp waits together, one elected lane issues ----------------
+            // (a branch on the lane number instead makes the twelve products of a tile take 740 cycles to issue, not 470)
+            // f32 accumulators; S^T: e4m3 both; O^T: f16 both, A (V) and B (weights) with their outer side contiguous
+            constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(C::S_COLS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint32_t idesc_o = (1u << 4) | (1u << 15) | (1u << 16) | ((uint32_t)(RP >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+            constexpr uint32_t hi_s = desc_hi(8 * C::ROWB, DH == 64 ? 4 : 2), hi_v = desc_hi(1024, 2);
+            constexpr uint32_t hi_p = desc_hi(8 * C::PROW, C::PROW == 128 ? 2 : C::PROW == 64 ? 4 : 6);
+            constexpr uint32_t v_lbo = DH == 64 ? 0 : 16384;  // (64 dims: the product's other 64 rows repeat them)
+            // O^T of the tile before: whether it is still to come, and begins or ends its span
+            bool pending = false, begins = false, ends = false;
+            const auto values = [&]() {
+                if (begins) wait(o_empty + 8 * ot.slot, ot.phase ^ 1);
+                wait(p_full + 8 * pt.slot, pt.phase);
+                wait(w_full + 8 * wt.slot, wt.phase);
+                tc_fence_after();
+                if (!dead && elected()) {
+                    const uint32_t va = desc_lo(smem_u32(v16 + wt.slot * C::V16), v_lbo), pa = desc_lo(smem_u32(s_p + pt.slot * C::PB));
+                    const uint32_t d = col_o(ot.slot);
 #pragma unroll
-                        for (int half = 0; half < C::HALVES; ++half)
+                    for (int half = 0; half < C::HALVES; ++half)
 #pragma unroll
-                            for (int ks = 0; ks < 8; ++ks)
-                                mma_tc<false>(d + (uint32_t)(half * RP), va + (uint32_t)(half * 2048 + ks * 128), hi_v,
-                                              pa + (uint32_t)(ks * C::PROW), hi_p, idesc_o, begins && ks == 0 ? 0u : 1u);
-                        tc_commit(p_empty + 8 * pt.slot);
-                        tc_commit(w_empty + 8 * wt.slot);
-                        if (ends) tc_commit(o_full + 8 * ot.slot);
-                    }
-                    pt.next();
-                    wt.next();
-                    if (ends) ot.next();
-                    pending = false;
-                };
-#pragma unroll 1
-                for (int si = 0; si < nseg; ++si) {
-                    const int n = segs[si].n;
-                    wait(q_full + 8 * qt.slot, qt.phase);
-#pragma unroll 1
-                    for (int i = 0; i < n; ++i) {
-                        wait(k_full + 8 * kt.slot, kt.phase);
-                        wait(s_empty + 8 * st.slot, st.phase ^ 1);
-                        tc_fence_after();
-                        if (!dead) {
-                            const uint32_t ka = desc_lo(smem_u32(k_ring + kt.slot * C::KT)), qa = desc_lo(smem_u32(s_q + qt.slot * C::QB));
-                            const uint32_t d = col_s(st.slot);
-#pragma unroll
-                            for (int ks = 0; ks < DH / 32; ++ks)
-                                mma_tc<true>(d, ka + (uint32_t)((ks >> 2) * (TCA_TILE * 8) + (ks & 3) * 2), hi_s,
-                                             qa + (uint32_t)((ks >> 2) * (2 * R * 8) + (ks & 3) * 2), hi_s, idesc_s, ks == 0 ? 0u : 1u);
-                            tc_commit(k_empty + 8 * kt.slot);
-                            tc_commit(s_full + 8 * st.slot);
-                            if (i == n - 1) tc_commit(q_empty + 8 * qt.slot);
-                        }
-                        mbar_arrive(s_full + 8 * st.slot);
-                        kt.next();
-                        st.next();
-                        if (pending) values();
-                        pending = true;
-                        begins = i == 0;
-                        ends = i == n - 1;
-                    }
-                    qt.next();
+                        for (int ks = 0; ks < 8; ++ks)
+                            mma_tc<false>(d + (uint32_t)(half * RP), va + (uint32_t)(half * 2048 + ks * 128), hi_v,
+                                          pa + (uint32_t)(ks * C::PROW), hi_p, idesc_o, begins && ks == 0 ? 0u : 1u);
+                    tc_commit(p_empty + 8 * pt.slot);
+                    tc_commit(w_empty + 8 * wt.slot);
+                    if (ends) tc_commit(o_full + 8 * ot.slot);
                 }
-                if (pending) values();
+                __syncwarp();
+                pt.next();
+                wt.next();
+                if (ends) ot.next();
+                pending = false;
+            };
+#pragma unroll 1
+            for (int si = 0; si < nseg; ++si) {
+                const int n = segs[si].n;
+                wait(q_full + 8 * qt.slot, qt.phase);
+#pragma unroll 1
+                for (int i = 0; i < n; ++i) {
+                    wait(k_full + 8 * kt.slot, kt.phase);
+                    wait(s_empty + 8 * st.slot, st.phase ^ 1);
+                    tc_fence_after();
+                    if (!dead && elected()) {
+                        const uint32_t ka = desc_lo(smem_u32(k_ring + kt.slot * C::KT)), qa = desc_lo(smem_u32(s_q + qt.slot * C::QB));
+                        const uint32_t d = col_s(st.slot);
+#pragma unroll
+                        for (int ks = 0; ks < DH / 32; ++ks)
+                            mma_tc<true>(d, ka + (uint32_t)((ks >> 2) * (TCA_TILE * 8) + (ks & 3) * 2), hi_s,
+                                         qa + (uint32_t)((ks >> 2) * (2 * R * 8) + (ks & 3) * 2), hi_s, idesc_s, ks == 0 ? 0u : 1u);
+                        tc_commit(s_full + 8 * st.slot);
+                        tc_commit(k_empty + 8 * kt.slot);
+                        if (i == n - 1) tc_commit(q_empty + 8 * qt.slot);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_full + 8 * st.slot);  // (passes on what this warp has seen: page words, factors)
+                    kt.next();
+                    st.next();
+                    if (pending) values();
+                    pending = true;
+                    begins = i == 0;
+                    ends = i == n - 1;
+                }
+                qt.next();
             }
+            if (pending) values();
         } else {
             // ---------------- queries: two e4m3 terms of each row ----------------
             constexpr int LPR = DH / 16, RPI = 32 / LPR;  // lanes a row, rows at a time
