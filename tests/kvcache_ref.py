@@ -95,10 +95,11 @@ def attention_bound(out, weight, spread, floor, dh, dtype):
     instruction may truncate), so a weight is off by a factor exp(+-d), d = spread * (dh + 8) * 2^-23,
     numerator and denominator each.  Weights: rounded to 11 bits (bf16 results) or to 22 (fp32), half
     a step each, 2^-11 and 2^-22; exp2 and the sums: 2^-20 together.  The result: half a step of its type.
-    f16 ends at 2^-24: a weight times its V block's scale is held as f16 with the row's largest at 2^7 or
-    above, so it is also off by half of 2^-24, 2^-32 of that largest; that error meets |code of V_j|, which
-    gives floor * 2^-32 over all keys (it counts where a dimension's V is zero for every key of weight)."""
+    f16 ends at 2^-24: a weight times its V block's scale is held as f16 with the row's largest at 2^3 or
+    above (fp32 queries: 2^7), so it is also off by half of 2^-24, 2^-28 (2^-32) of that largest; that error
+    meets |code of V_j|, which gives floor * 2^-28 (2^-32) over all keys (it counts where a dimension's V is
+    zero for every key of weight)."""
     d = spread[..., None] * (dh + 8) * 2.0 ** -23
     w = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
     half = torch.finfo(dtype).eps / 2
-    return out.abs() * half + weight * (1 + half) * (2 * torch.expm1(d) + w + 2.0 ** -20) + floor * 2.0 ** -32 + 1e-30
+    return out.abs() * half + weight * (1 + half) * (2 * torch.expm1(d) + w + 2.0 ** -20) + floor * (2.0 ** -28 if dtype == torch.bfloat16 else 2.0 ** -32) + 1e-30

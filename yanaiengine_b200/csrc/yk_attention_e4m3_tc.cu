@@ -19,9 +19,11 @@
 // hold them exactly (to 2^-21 of a row's largest value at least), as separate
 // columns of one product.  V converts once for all rows of the tile (R up to 64).
 //
-// Weights as in the other kernel: p = 2^(x + e_V - m), f16 with room for 2^8
-// before the reference m moves; m is common to the CTA, kept lazily: it moves
-// when a weight would pass 2^15, and at a span's first keys.
+// Weights as in the other kernel: p = 2^(x + e_V - m), f16.  The reference m is
+// common to the CTA and kept lazily: it is set 2^3 below a row's first weights
+// and moves when one would pass 2^15 (each move waits for the products before it
+// and rescales O^T in TMEM).  What lies 2^-28 below a row's largest weight is
+// lost: f16 ends at 2^-25, rounded.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -85,10 +87,17 @@ __device__ __forceinline__ void tmem_ld(uint32_t a, uint32_t* r) {
     }
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3])
-                 : "memory");
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t* r) {
+    if constexpr (N >= 8) {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                     "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                     : "memory");
+        if constexpr (N > 8) tmem_st<N - 8>(a + 8, r + 8);
+    } else {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                     : "memory");
+    }
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Shared-memory matrix descriptors (sm_100), as two words: the low one holds the
@@ -189,6 +198,15 @@ __device__ __noinline__ void note_nans(uint32_t cells, int dim0, int key, int po
     }
 }
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {  // (does not wait)
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool elected() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -298,7 +316,13 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
     // per role, through all rounds
     bool dead = false;  // a bounded wait ran out: the role goes through the motions without touching memory
     const auto wait = [&](uint32_t bar, int parity) {
-        if (!dead && !mbar_try_wait(bar, (uint32_t)parity)) dead = !wait_longer(bar, (uint32_t)parity, p.err);
+        if (!dead && !mbar_test(bar, (uint32_t)parity)) dead = !wait_longer(bar, (uint32_t)parity, p.err);
+    };
+    // two at once: the first looks at both go out together (one that finds its barrier ready takes ~100 cycles)
+    const auto wait2 = [&](uint32_t bar_a, int parity_a, uint32_t bar_b, int parity_b) {
+        const bool a = mbar_test(bar_a, (uint32_t)parity_a), b = mbar_test(bar_b, (uint32_t)parity_b);
+        if (!dead && !a) dead = !wait_longer(bar_a, (uint32_t)parity_a, p.err);
+        if (!dead && !b) dead = !wait_longer(bar_b, (uint32_t)parity_b, p.err);
     };
     Turn<NK> kt;
     Turn<NV> vt;
@@ -316,7 +340,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
         const int nseg = min(A8_SEGS, work.nspans - seg0);
         if (warp < 8) {
             // ---------------- softmax: key 32 * quad + lane of each tile, rows r0 .. r0 + RH - 1 ----------------
-            constexpr int RH = C::RH, BATCH = RH > 16 ? RH / 2 : RH;  // rows read from TMEM at a time
+            constexpr int RH = C::RH, BATCH = RH > 16 ? 8 : RH;  // rows read from TMEM at a time
             const int quad = warp & 3, r0 = (warp >> 2) * RH, key = 32 * quad + lane;
             const uint32_t lanes = (uint32_t)(32 * quad) << 16;
             // this key's weights in P, [key][row], 16-byte chunks swizzled by the key
@@ -343,6 +367,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     const int j0 = (sg.page + TCA_PAGES * i) * 16;
                     wait(s_full + 8 * st.slot, st.phase);
                     tc_fence_after();
+                    const bool p_free = mbar_test(p_empty + 8 * pt.slot, (uint32_t)(pt.phase ^ 1));
                     const int info = s_info[(tile & (C::INFO - 1)) * TCA_PAGES + 2 * quad + (lane >> 4)];
                     const bool here = info >= 0;
                     const int ek = here ? (info & 255) - 128 : 0, ev = here ? (info >> 8) - 128 : 0;
@@ -357,29 +382,33 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                         uint32_t x[BATCH], y[BATCH];
                         tmem_ld<BATCH>(at + (uint32_t)b0, x);
                         tmem_ld<BATCH>(at + (uint32_t)(R + b0), y);
+                        float4 f[BATCH / 4], m[BATCH / 4];  // (these come while the scores do)
+#pragma unroll
+                        for (int n = 0; n < BATCH / 4; ++n) {
+                            f[n] = *reinterpret_cast<const float4*>(rf + b0 + 4 * n);
+                            m[n] = *reinterpret_cast<const float4*>(s_neg + r0 + b0 + 4 * n);
+                        }
                         tmem_wait_ld();
 #pragma unroll
-                        for (int n = 0; n < BATCH; n += 2)
-                            d[(b0 + n) / 2] = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f),
-                                                   make_float2(__uint_as_float(x[n]), __uint_as_float(x[n + 1])));
+                        for (int n = 0; n < BATCH; n += 2) {
+                            const float4 ff = f[n / 4], mm = m[n / 4];
+                            const float2 s = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f),
+                                                  make_float2(__uint_as_float(x[n]), __uint_as_float(x[n + 1])));
+                            const float2 r = n & 2 ? make_float2(ff.z, ff.w) : make_float2(ff.x, ff.y);
+                            const float2 c = add2(shift, n & 2 ? make_float2(mm.z, mm.w) : make_float2(mm.x, mm.y));
+                            // (soft-capped scores are capped, then shifted, below)
+                            d[(b0 + n) / 2] = p.cap <= 0.f ? fma2(mul2(s, fk2), r, c) : mul2(mul2(s, fk2), r);
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s_empty + 8 * st.slot);
                     st.next();
-                    if (p.cap <= 0.f) {
-#pragma unroll
-                        for (int n = 0; n < RH; n += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(rf + n), m = *reinterpret_cast<const float4*>(s_neg + r0 + n);
-                            d[n / 2] = fma2(mul2(d[n / 2], fk2), make_float2(f.x, f.y), add2(shift, make_float2(m.x, m.y)));
-                            d[n / 2 + 1] = fma2(mul2(d[n / 2 + 1], fk2), make_float2(f.z, f.w), add2(shift, make_float2(m.z, m.w)));
-                        }
-                    } else {
+                    if (p.cap > 0.f) {
 #pragma unroll
                         for (int n = 0; n < RH; n += 2) {
-                            const float2 f = *reinterpret_cast<const float2*>(rf + n), m = *reinterpret_cast<const float2*>(s_neg + r0 + n);
-                            const float2 x = mul2(mul2(d[n / 2], fk2), f);
-                            d[n / 2] = add2(make_float2(cap_score(p, x.x), cap_score(p, x.y)), add2(shift, m));
+                            const float2 m = *reinterpret_cast<const float2*>(s_neg + r0 + n);
+                            d[n / 2] = add2(make_float2(cap_score(p, d[n / 2].x), cap_score(p, d[n / 2].y)), add2(shift, m));
                         }
                     }
                     if (!plain) {
@@ -400,11 +429,13 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     for (int n = 0; n < RH / 2; ++n) top = fmaxf(top, fmaxf(d[n].x, d[n].y));
                     // move the references: at a row's first keys, and before a weight would pass 2^15
                     if (softmax_or(force || top > 15.f)) {
+                        float most = 0.f;  // lane n: the warp's largest of row r0 + n
 #pragma unroll
                         for (int n = 0; n < RH; ++n) {
                             const float x = warp_fmax(n & 1 ? d[n / 2].y : d[n / 2].x);
-                            if (lane == n) s_mx[quad * R + r0 + n] = x;
+                            most = lane == n ? x : most;
                         }
+                        if (lane < RH) s_mx[quad * R + r0 + lane] = most;
                         softmax_bar();
                         bool unset = false;
                         if (threadIdx.x < R) {
@@ -412,7 +443,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             const float x = fmaxf(fmaxf(s_mx[n], s_mx[R + n]), fmaxf(s_mx[2 * R + n], s_mx[3 * R + n]));
                             const float was = -s_neg[n];
                             const bool set = s_set[n] != 0;
-                            const float now = x == -INFINITY ? was : set ? fmaxf(was, was + (x - 7.f)) : was + (x - 7.f);
+                            const float now = x == -INFINITY ? was : set ? fmaxf(was, was + (x - 3.f)) : was + (x - 3.f);
                             s_f[n] = set ? ex2(was - now) : 1.f;
                             s_dm[n] = was - now;
                             s_neg[n] = -now;
@@ -433,22 +464,24 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             wait(p_empty + 8 * (pt.slot ^ 1), pt.slot ? pt.phase : pt.phase ^ 1);
                             tc_fence_after();
 #pragma unroll 1
-                            for (int n = 0; n < C::HALVES * RH; n += 4) {
-                                const int n0 = r0 + n % RH;
-                                const uint32_t o_at = col_o(ot.slot) + lanes + (uint32_t)((n / RH) * RP + n0);
-                                uint32_t x[4];
-                                tmem_ld<4>(o_at, x);
-                                tmem_wait_ld();
+                            for (int half = 0; half < C::HALVES; ++half) {
+                                const uint32_t o_at = col_o(ot.slot) + lanes + (uint32_t)(half * RP + r0);
+#pragma unroll 1
+                                for (int n = 0; n < RH; n += BATCH) {
+                                    uint32_t x[BATCH];
+                                    tmem_ld<BATCH>(o_at + (uint32_t)n, x);
+                                    tmem_wait_ld();
 #pragma unroll
-                                for (int z = 0; z < 4; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * s_f[n0 + z]);
-                                tmem_st4(o_at, x);
+                                    for (int z = 0; z < BATCH; ++z) x[z] = __float_as_uint(__uint_as_float(x[z]) * s_f[r0 + n + z]);
+                                    tmem_st<BATCH>(o_at + (uint32_t)n, x);
+                                }
                             }
                             tmem_wait_st();
                             tc_fence_before();
                         }
                     }
                     // weights
-                    wait(p_empty + 8 * pt.slot, pt.phase ^ 1);
+                    if (!p_free) wait(p_empty + 8 * pt.slot, pt.phase ^ 1);
                     const uint32_t pa = p_at + (uint32_t)(pt.slot * C::PB);
                     if (!dead) {
                         constexpr int PER = RH % 8 == 0 ? 8 : 4;  // rows a store
@@ -515,8 +548,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
 #pragma unroll 1
                 for (int i = 0; i < sg.n; ++i, ++tile) {
                     const int j0 = (sg.page + TCA_PAGES * i) * 16;
-                    wait(v_full + 8 * vt.slot, vt.phase);
-                    wait(w_empty + 8 * wt.slot, wt.phase ^ 1);
+                    wait2(v_full + 8 * vt.slot, vt.phase, w_empty + 8 * wt.slot, wt.phase ^ 1);
                     const int* const info = s_info + C::INFO * TCA_PAGES + (tile & (C::INFO - 1)) * TCA_PAGES;
                     const int4 i0 = *reinterpret_cast<const int4*>(info), i1 = *reinterpret_cast<const int4*>(info + 4);
                     const bool plain = all_seen(p, sg, pos_last, j0) && (i0.x | i0.y | i0.z | i0.w | i1.x | i1.y | i1.z | i1.w) >= 0;
@@ -716,8 +748,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
             bool pending = false, begins = false, ends = false;
             const auto values = [&]() {
                 if (begins) wait(o_empty + 8 * ot.slot, ot.phase ^ 1);
-                wait(p_full + 8 * pt.slot, pt.phase);
-                wait(w_full + 8 * wt.slot, wt.phase);
+                wait2(p_full + 8 * pt.slot, pt.phase, w_full + 8 * wt.slot, wt.phase);
                 tc_fence_after();
                 if (!dead && elected()) {
                     const uint32_t va = desc_lo(smem_u32(v16 + wt.slot * C::V16), v_lbo), pa = desc_lo(smem_u32(s_p + pt.slot * C::PB));
@@ -744,8 +775,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                 wait(q_full + 8 * qt.slot, qt.phase);
 #pragma unroll 1
                 for (int i = 0; i < n; ++i) {
-                    wait(k_full + 8 * kt.slot, kt.phase);
-                    wait(s_empty + 8 * st.slot, st.phase ^ 1);
+                    wait2(k_full + 8 * kt.slot, kt.phase, s_empty + 8 * st.slot, st.phase ^ 1);
                     tc_fence_after();
                     if (!dead && elected()) {
                         const uint32_t ka = desc_lo(smem_u32(k_ring + kt.slot * C::KT)), qa = desc_lo(smem_u32(s_q + qt.slot * C::QB));
