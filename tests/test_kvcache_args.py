@@ -111,8 +111,26 @@ def test_wrapper_checks_tensors_on_the_host():
 
     pool = torch.zeros(4, 2, 2, 2, 16, 64, dtype=torch.uint8)
     with pytest.raises(ValueError, match="not on cuda"):
-        abi.kv_pages(pool, torch.zeros(4, 2, 2, 2, dtype=torch.uint8), 0)
-    with pytest.raises(ValueError, match="needs scales"):
-        abi.kv_pages(pool, None, 0)
+        abi._pages(pool, torch.zeros(4, 2, 2, 2, dtype=torch.uint8), 0)
     with pytest.raises(ValueError, match="must be"):
-        abi.kv_pages(pool[:, :, :1], None, 0)
+        abi._pages(pool[:, :, :1], None, 0)
+    with pytest.raises(ValueError, match="not on cuda"):
+        abi.kv_append(pool, None, 0, torch.zeros(1, 256), torch.zeros(1, 2, 64), torch.zeros(1, dtype=torch.int32), None,
+                      None, None, 1e-5, None, 2)
+
+
+def test_packed_arguments_match_the_structures():
+    a = attention_args(layer=1, window=7, scale=0.5, cap=2.0, workspace_bytes=77)
+    p = a.pages
+    raw = abi._ATTENTION.pack(p.data, p.scales, p.kind, p.num_blocks, p.n_layers, p.n_kv_heads, p.head_dim, a.layer, a.T, a.B,
+                              a.n_heads, a.dtype, a.max_blocks, a.max_new, a.window, a.scale, a.cap, a.q, a.q_stride, a.out,
+                              a.out_stride, a.q_starts, a.context_lens, a.block_tables, a.workspace, a.workspace_bytes, a.err)
+    b = abi.AttentionE4M3Args.from_buffer_copy(raw)
+    assert all(getattr(a, f) == getattr(b, f) for f, _ in a._fields_[1:])
+    assert all(getattr(a.pages, f) == getattr(b.pages, f) for f, _ in p._fields_)
+    a = append_args(layer=1, eps=0.5)
+    raw = abi._APPEND.pack(p.data, p.scales, p.kind, p.num_blocks, p.n_layers, p.n_kv_heads, p.head_dim, a.layer, a.T, a.n_heads,
+                           a.src_dtype, a.q_dtype, a.eps, a.qkv, a.qkv_stride, a.q_out, a.q_stride, a.slots, a.rope, a.q_gain,
+                           a.k_gain, a.err)
+    b = abi.KVAppendArgs.from_buffer_copy(raw)
+    assert all(getattr(a, f) == getattr(b, f) for f, _ in a._fields_[1:])

@@ -6,6 +6,7 @@ missing this raises instead of falling back to anything else.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -145,8 +146,8 @@ _PROTOS = {
     "yk_tp_allgather_u32": (C.c_int32, [_P, _U32P, C.c_int32, _U32P]),
     "yk_spec_verify_logits_noalloc": (C.c_int32, [C.c_int32, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                                   C.c_float, C.c_uint64, C.c_uint32, _P, _P]),
-    "yk_kv_append": (C.c_int32, [C.c_int32, _P, C.POINTER(KVAppendArgs)]),
-    "yk_attention_e4m3": (C.c_int32, [C.c_int32, _P, C.POINTER(AttentionE4M3Args)]),
+    "yk_kv_append": (C.c_int32, [C.c_int32, _P, _P]),
+    "yk_attention_e4m3": (C.c_int32, [C.c_int32, _P, _P]),
     "yk_attention_e4m3_workspace": (C.c_int32, [C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
     # include/yk_testing.h
     "ykt_gemm_bf16": (C.c_int32, [_P, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16), C.c_int32, C.c_int32,
@@ -318,69 +319,92 @@ def tp_unique_id() -> bytes:
 # ---------------------------------------------------------------------------
 # Operators on a paged KV cache held in torch CUDA tensors (include/yk.h).
 # Tensors are used in place, on the device they share and on its current torch
-# stream (or `stream`, a cudaStream_t); nothing is copied, cast or kept.
+# stream (or `stream`, a cudaStream_t); nothing is copied, cast or kept.  The
+# argument structures are packed as bytes (a third of the time of filling a
+# ctypes.Structure field by field, on calls that take a few microseconds).
 # ---------------------------------------------------------------------------
+_APPEND = struct.Struct("@2P5i4x5ifPqPq5P")
+_ATTENTION = struct.Struct("@2P5i4x8i2fPqPq4PQP")
+assert _APPEND.size == C.sizeof(KVAppendArgs) and _ATTENTION.size == C.sizeof(AttentionE4M3Args)
+_INTS, _FLOATS = frozenset(("torch.int32", "torch.uint32")), {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
+_dtypes: dict = {}  # torch dtype -> (name, element size)
+
+
+def _kind(t):
+    d = t.dtype
+    k = _dtypes.get(d)
+    if k is None:
+        k = _dtypes[d] = (str(d), t.element_size())
+    return k
+
+
 def _code(t, name: str) -> int:
-    import torch
-
-    if t.dtype == torch.bfloat16:
-        return DTYPE_BF16
-    if t.dtype == torch.float32:
-        return DTYPE_F32
-    raise ValueError(f"{name}: float32 or bfloat16, not {t.dtype}")
+    c = _FLOATS.get(_kind(t)[0])
+    if c is None:
+        raise ValueError(f"{name}: float32 or bfloat16, not {t.dtype}")
+    return c
 
 
-def _address(t, name: str, device: int, size: int, numel: int | None = None, whole: bool = False):
-    """data_ptr of a contiguous tensor on `device` with elements of `size` bytes (None: null);
-    whole: of integers."""
-    if t is None:
-        return None
-    if whole and t.dtype.is_floating_point:
-        raise ValueError(f"{name} must hold 32-bit integers")
-    if not t.is_cuda or t.get_device() != device:
-        raise ValueError(f"{name} is not on cuda:{device}")
-    if t.element_size() != size or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with {size}-byte elements")
-    if numel is not None and t.numel() != numel:
-        raise ValueError(f"{name} must have {numel} elements, not {t.numel()}")
+def _ints(t, name: str, device: int, numel: int = -1) -> int:
+    if t.get_device() != device or not t.is_contiguous() or _kind(t)[0] not in _INTS or 0 <= numel != t.numel():
+        raise ValueError(f"{name} must be contiguous 32-bit integers on cuda:{device}" + (f", {numel} of them" if numel >= 0 else ""))
     return t.data_ptr()
 
 
-def kv_pages(pool, scales, device: int) -> KVPages:
-    """pool [blocks, layers, 2, kv heads, 16, head_dim]: 1-byte elements with scales
+def _reals(t, name: str, device: int, numel: int) -> int:
+    if t is None:
+        return 0
+    if t.get_device() != device or not t.is_contiguous() or _kind(t)[0] != "torch.float32" or numel != t.numel():
+        raise ValueError(f"{name} must be {numel} contiguous float32 values on cuda:{device}")
+    return t.data_ptr()
+
+
+def _pages(pool, scales, device: int) -> tuple:
+    """The fields of yk_kv_pages.  pool [blocks, layers, 2, kv heads, 16, head_dim]: 1-byte elements with scales
     [blocks, layers, 2, kv heads] (1-byte elements), or fp32 / bf16 and scales None."""
-    if pool.dim() != 6 or pool.shape[2] != 2 or pool.shape[4] != BLOCK_SIZE:
+    if pool.dim() != 6:
         raise ValueError("pool must be [blocks, layers, 2, kv heads, 16, head_dim]")
-    n, layers, _, g, _, dh = pool.shape
-    size = pool.element_size()
-    if size == 1:
-        if scales is None:
-            raise ValueError("a pool of 8-bit cells needs scales")
-        kind = KV_E4M3
-    else:
-        kind = KV_F32 if _code(pool, "pool") == DTYPE_F32 else KV_BF16
-    return KVPages(_address(pool, "pool", device, size), _address(scales, "scales", device, 1, n * layers * 2 * g),
-                   kind, n, layers, g, dh)
+    n, layers, two, g, slots, dh = pool.shape
+    if two != 2 or slots != BLOCK_SIZE:
+        raise ValueError("pool must be [blocks, layers, 2, kv heads, 16, head_dim]")
+    if pool.get_device() != device or device < 0 or not pool.is_contiguous():
+        raise ValueError(f"pool is not on cuda:{device}, or not contiguous")
+    if _kind(pool)[1] != 1:
+        if scales is not None:
+            raise ValueError("scales belong to a pool of 8-bit cells")
+        return pool.data_ptr(), 0, KV_F32 if _code(pool, "pool") == DTYPE_F32 else KV_BF16, n, layers, g, dh
+    if scales is None:
+        raise ValueError("a pool of 8-bit cells needs scales")
+    if scales.get_device() != device or not scales.is_contiguous() or _kind(scales)[1] != 1 or scales.numel() != n * layers * 2 * g:
+        raise ValueError(f"scales must be [blocks, layers, 2, kv heads] contiguous bytes on cuda:{device}")
+    return pool.data_ptr(), scales.data_ptr(), KV_E4M3, n, layers, g, dh
 
 
-def _rows(t, name: str, device: int, tokens: int, heads: int, dh: int):
+def _rows(t, name: str, device: int, tokens: int, heads: int, dh: int) -> tuple:
     """(address, elements between tokens) of [tokens, heads, head_dim] (or [tokens, heads * head_dim])."""
-    if not t.is_cuda or t.get_device() != device:
-        raise ValueError(f"{name} is not on cuda:{device}")
-    s = t.stride()
-    tail = s[1:] == (dh, 1) and t.shape[1:] == (heads, dh) if t.dim() == 3 else t.dim() == 2 and \
-        s[1] == 1 and t.shape[1] == heads * dh
-    if t.shape[0] != tokens or not tail:
-        raise ValueError(f"{name} must be [{tokens}, {heads}, {dh}] with contiguous rows")
+    s, shape = t.stride(), t.shape
+    if len(s) == 3:
+        good = s[1] == dh and s[2] == 1 and shape[1] == heads and shape[2] == dh
+    else:
+        good = len(s) == 2 and s[1] == 1 and shape[1] == heads * dh
+    if not good or shape[0] != tokens or t.get_device() != device:
+        raise ValueError(f"{name} must be [{tokens}, {heads}, {dh}] on cuda:{device}, its rows contiguous")
     return t.data_ptr(), (s[0] if tokens > 1 else heads * dh)
 
 
+_raw_stream = None
+
+
 def _stream(device: int, stream):
-    if stream is None:
+    global _raw_stream
+    if stream is not None:
+        return stream
+    if _raw_stream is None:
         import torch
 
-        return torch.cuda.current_stream(device).cuda_stream
-    return stream
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 def kv_append(pool, scales, layer: int, qkv, q_out, slots, rope, q_gain, k_gain, eps: float, err, heads: int,
@@ -389,14 +413,15 @@ def kv_append(pool, scales, layer: int, qkv, q_out, slots, rope, q_gain, k_gain,
     queries to q_out [T, heads, head_dim], keys and values to cache slots [T] (int32) of `layer`.
     rope [T, head_dim / 2, 2], q_gain / k_gain [head_dim]: fp32 or None; err: int32 [1] or None."""
     dev = qkv.get_device()
-    pages = kv_pages(pool, scales, dev)
-    g, dh, n = pages.n_kv_heads, pages.head_dim, slots.numel()
-    a = KVAppendArgs(pages, layer, n, heads, _code(qkv, "qkv"), _code(q_out, "q_out"), eps,
+    pages = _pages(pool, scales, dev)
+    g, dh, n = pages[5], pages[6], slots.numel()
+    a = _APPEND.pack(*pages, layer, n, heads, _code(qkv, "qkv"), _code(q_out, "q_out"), eps,
                      *_rows(qkv, "qkv", dev, n, heads + 2 * g, dh), *_rows(q_out, "q_out", dev, n, heads, dh),
-                     _address(slots, "slots", dev, 4, whole=True), _address(rope, "rope", dev, 4, n * dh),
-                     _address(q_gain, "q_gain", dev, 4, dh), _address(k_gain, "k_gain", dev, 4, dh),
-                     _address(err, "err", dev, 4))
-    check(lib().yk_kv_append(dev, _stream(dev, stream), C.byref(a)))
+                     _ints(slots, "slots", dev), _reals(rope, "rope", dev, n * dh), _reals(q_gain, "q_gain", dev, dh),
+                     _reals(k_gain, "k_gain", dev, dh), 0 if err is None else _ints(err, "err", dev))
+    st = lib().yk_kv_append(dev, _stream(dev, stream), a)
+    if st:
+        check(st)
 
 
 def attention_e4m3(q, out, pool, scales, layer: int, q_starts, context_lens, block_tables, workspace, err, *,
@@ -405,21 +430,23 @@ def attention_e4m3(q, out, pool, scales, layer: int, q_starts, context_lens, blo
     q_starts [B + 1], context_lens [B], block_tables [B, max_blocks]: int32; workspace: bytes (at least
     attention_e4m3_workspace(...)), zeroed once by the caller; err: int32 [1] or None."""
     dev = q.get_device()
-    pages = kv_pages(pool, scales, dev)
+    pages = _pages(pool, scales, dev)
     if q.dim() != 3 or block_tables.dim() != 2:
         raise ValueError("q must be [T, heads, head_dim], block_tables [B, max_blocks]")
     n, heads, dh = q.shape
     B, width = block_tables.shape
-    if dh != pages.head_dim or out.dtype != q.dtype:
+    if dh != pages[6] or out.dtype != q.dtype:
         raise ValueError("q, out and the pool disagree on head_dim or dtype")
-    a = AttentionE4M3Args(pages, layer, n, B, heads, _code(q, "q"), width, max_new, window, scale, cap,
-                          *_rows(q, "q", dev, n, heads, dh), *_rows(out, "out", dev, n, heads, dh),
-                          _address(q_starts, "q_starts", dev, 4, B + 1, True),
-                          _address(context_lens, "context_lens", dev, 4, B, True),
-                          _address(block_tables, "block_tables", dev, 4, whole=True),
-                          _address(workspace, "workspace", dev, workspace.element_size()),
-                          workspace.numel() * workspace.element_size(), _address(err, "err", dev, 4))
-    check(lib().yk_attention_e4m3(dev, _stream(dev, stream), C.byref(a)))
+    if workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on cuda:{dev}")
+    a = _ATTENTION.pack(*pages, layer, n, B, heads, _code(q, "q"), width, max_new, window, scale, cap,
+                        *_rows(q, "q", dev, n, heads, dh), *_rows(out, "out", dev, n, heads, dh),
+                        _ints(q_starts, "q_starts", dev, B + 1), _ints(context_lens, "context_lens", dev, B),
+                        _ints(block_tables, "block_tables", dev), workspace.data_ptr(), workspace.nbytes,
+                        0 if err is None else _ints(err, "err", dev))
+    st = lib().yk_attention_e4m3(dev, _stream(dev, stream), a)
+    if st:
+        check(st)
 
 
 def attention_e4m3_workspace(head_dim: int, device: int = 0) -> int:

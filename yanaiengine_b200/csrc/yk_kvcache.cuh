@@ -69,7 +69,7 @@ inline cudaError_t launch_on(cudaStream_t stream, bool pdl, void (*kernel)(KArgs
 // current device).
 yk_status kv_pages_check(const yk_kv_pages& p, int32_t layer);
 yk_status kv_append_check(const yk_kv_append_args& a);
-yk_status kv_append_launch(cudaStream_t stream, bool pdl, const yk_kv_append_args& a);
+yk_status kv_append_launch(cudaStream_t stream, bool pdl, int num_sms, const yk_kv_append_args& a);
 yk_status attention_e4m3_check(const yk_attention_e4m3_args& a);  // (all but the workspace's size)
 yk_status attention_e4m3_launch(cudaStream_t stream, bool pdl, int num_sms, const yk_attention_e4m3_args& a);
 size_t attention_e4m3_ws_bytes(int num_sms, int head_dim);
