@@ -25,67 +25,54 @@ struct AppendParams {
     float eps;
 };
 
-// N consecutive elements at p (N * size <= 16 bytes per load) as fp32.
-template <int N>
-__device__ __forceinline__ void load_row(const float* p, float (&v)[N]) {
-    if constexpr (N == 2) {
-        const float2 a = *reinterpret_cast<const float2*>(p);
-        v[0] = a.x; v[1] = a.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p + i);
-            v[i] = a.x; v[i + 1] = a.y; v[i + 2] = a.z; v[i + 3] = a.w;
-        }
-    }
+// Eight consecutive elements as fp32, and back.
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
-template <int N>
-__device__ __forceinline__ void load_row(const __nv_bfloat16* p, float (&v)[N]) {
-    uint32_t w[N / 2];
-    if constexpr (N == 2) {
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
-    } else if constexpr (N == 4) {
-        const uint2 a = *reinterpret_cast<const uint2*>(p);
-        w[0] = a.x; w[1] = a.y;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    }
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
         v[2 * i] = __uint_as_float(w[i] << 16);
         v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-template <int N, typename AT>
-__device__ __forceinline__ void store_row(AT* p, const float (&v)[N]) {
-    if constexpr (N == 2) {
-        store2(p, v[0], v[1]);
-    } else {
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < N; i += 4) store4(p + i, v[i], v[i + 1], v[i + 2], v[i + 3]);
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&x);
     }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One head of one token, spread over a warp (lane: N = DH / 32 consecutive
-// dims): the norm over the head, then the rotation of its pairs.
-template <int DH, int N>
-__device__ __forceinline__ void norm_rotate(const AppendParams& p, const float* gain, int t, int lane, float (&v)[N]) {
-    if (gain) {
+// One head of one token, spread over DH / 8 lanes (8 consecutive dims each: a
+// warp holds 32 * 8 / DH rows): the norm over the head, then the rotation of its
+// pairs.  gain, cs: this lane's gains and (cos, sin) of its 4 pairs.  Every lane
+// of the warp calls it.
+template <int DH>
+__device__ __forceinline__ void norm_rotate(bool norm, bool turn, float eps, const float (&gain)[8], const float (&cs)[8], float (&v)[8]) {
+    if (norm) {
         float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) ss = fmaf(v[i], v[i], ss);
-        const float inv = rsqrtf(warp_sum_f(ss) * (1.0f / DH) + p.eps);
-        float g[N];
-        load_row<N>(gain + lane * N, g);
+        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] * inv * g[i];
+        for (int o = DH / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss * (1.0f / DH) + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * gain[i];
     }
-    if (p.rope) {
-        float cs[N];  // (cos, sin) of N / 2 pairs
-        load_row<N>(reinterpret_cast<const float*>(p.rope + (size_t)t * (DH / 2)) + lane * N, cs);
+    if (turn) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
+        for (int i = 0; i < 8; i += 2) {
             const float2 r = rope_rot(v[i], v[i + 1], cs[i], cs[i + 1]);
             v[i] = r.x;
             v[i + 1] = r.y;
@@ -94,42 +81,55 @@ __device__ __forceinline__ void norm_rotate(const AppendParams& p, const float* 
 }
 
 // The rows that stand alone: query heads, and with fp32 / bf16 pools key and
-// value heads too.  A warp takes ROWS of them, consecutive in (token, head)
-// order, their loads in flight together.
-template <typename SRC, typename DST, bool E4M3, int DH, int ROWS>
-__device__ __forceinline__ void append_rows(const AppendParams& p, long long first, int lane) {
-    constexpr int N = DH / 32;
-    const int all = p.H + 2 * p.G, heads = E4M3 ? p.H : all;
-    int t = (int)(first / heads), h = (int)(first - (long long)t * heads);
-    float v[ROWS][N];
-    int ts[ROWS], hs[ROWS], slot[ROWS];
+// value heads too.  A warp takes STEPS * (32 * 8 / DH) consecutive heads of one
+// token: their loads go out together, angles and gains are loaded once.
+template <typename SRC, typename DST, bool E4M3, int DH, int STEPS>
+__device__ __forceinline__ void append_rows(const AppendParams& p, long long task, int lane) {
+    constexpr int LPR = DH / 8, RPW = 32 / LPR;
+    const int heads = E4M3 ? p.H : p.H + 2 * p.G, chunks = (heads + STEPS * RPW - 1) / (STEPS * RPW);
+    const int t = (int)(task / chunks), h0 = (int)(task - (long long)t * chunks) * (STEPS * RPW) + lane / LPR, d = lane % LPR * 8;
+    if (t >= p.T) return;
+    const int slot = p.slots[t];
+    const SRC* const src = reinterpret_cast<const SRC*>(p.qkv) + (size_t)t * p.qkv_stride + d;
+    float v[STEPS][8], cs[8], gain[8];
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        ts[i] = t;
-        hs[i] = h;
-        slot[i] = -1;
-        if (t < p.T) {
-            slot[i] = p.slots[t];
-            load_row<N>(reinterpret_cast<const SRC*>(p.qkv) + (size_t)t * p.qkv_stride + (size_t)h * DH + lane * N, v[i]);
-        }
-        if (++h == heads) {
-            h = 0;
-            ++t;
-        }
+    for (int i = 0; i < STEPS; ++i) {
+        const int h = h0 + i * RPW;
+        if (h < heads) load8(src + (size_t)h * DH, v[i]);
     }
+    if (p.rope) load8(reinterpret_cast<const float*>(p.rope + (size_t)t * (DH / 2)) + d, cs);
+    if (E4M3 && p.q_gain) load8(p.q_gain + d, gain);
+    if (slot < 0) return;  // padding
+    const bool inside = (slot >> 4) < p.num_blocks;
+    if (!inside && lane == 0 && h0 == 0) raise_err(p.err, YK_DEV_ERR_BOUNDS);
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        if (slot[i] < 0) continue;  // padding
-        const bool query = hs[i] < p.H;
-        if (query || hs[i] < p.H + p.G) norm_rotate<DH, N>(p, query ? p.q_gain : p.k_gain, ts[i], lane, v[i]);
-        if (query) {
-            store_row<N>(reinterpret_cast<DST*>(p.q_out) + (size_t)ts[i] * p.q_stride + (size_t)hs[i] * DH + lane * N, v[i]);
-        } else if ((slot[i] >> 4) < p.num_blocks) {
-            store_row<N>(reinterpret_cast<DST*>(p.pool) + (size_t)(slot[i] >> 4) * p.block_cells + p.layer_off +
-                             ((size_t)(hs[i] - p.H) * 16 + (slot[i] & 15)) * DH + lane * N,
-                         v[i]);
+    for (int i = 0; i < STEPS; ++i) {
+        const int h = h0 + i * RPW;
+        bool norm = p.q_gain != nullptr, turn = p.rope != nullptr;
+        if constexpr (!E4M3) {
+            // (rows of a warp may be of different kinds: those without a norm or a turn get gains and angles that
+            // change nothing, applied by selection)
+            const float* const g = h < p.H ? p.q_gain : h < p.H + p.G ? p.k_gain : nullptr;
+            const bool mine = g != nullptr;
+            if (mine) load8(g + d, gain);
+            float w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = v[i][k];
+            norm_rotate<DH>(__any_sync(0xffffffffu, mine), false, p.eps, gain, cs, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[i][k] = mine ? w[k] : v[i][k];
+            norm = false;
+            turn = turn && h < p.H + p.G;
         }
-        if (hs[i] == 0 && lane == 0 && (slot[i] >> 4) >= p.num_blocks) raise_err(p.err, YK_DEV_ERR_BOUNDS);
+        norm_rotate<DH>(norm, turn, p.eps, gain, cs, v[i]);
+        if (h >= heads) continue;
+        if (h < p.H) {
+            store8(reinterpret_cast<DST*>(p.q_out) + (size_t)t * p.q_stride + (size_t)h * DH + d, v[i]);
+        } else if (inside) {
+            store8(reinterpret_cast<DST*>(p.pool) + (size_t)(slot >> 4) * p.block_cells + p.layer_off +
+                       ((size_t)(h - p.H) * 16 + (slot & 15)) * DH + d,
+                   v[i]);
+        }
     }
 }
 
@@ -138,8 +138,9 @@ __device__ __forceinline__ void append_rows(const AppendParams& p, long long fir
 // that follow it.  Their values wait in shared memory (fp32) for the scale.
 template <typename SRC, int DH>
 __device__ __forceinline__ void append_block(const AppendParams& p, int t, int slot, int h, int lane, float* stage) {
-    constexpr int N = DH / 32;
+    constexpr int LPR = DH / 8, RPW = 32 / LPR;
     const bool key = h < p.G;
+    const int sub = lane / LPR, d = lane % LPR * 8;
     // the block's rows from here on: lane i holds the i-th one's row and offset
     int run = 0, row_i = t, off_i = 0;
     for (int at = t; at < p.T; at += 32) {
@@ -165,29 +166,36 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int t, int s
     const uint32_t older = ((1u << (31 - __clz(fresh))) - 1) & ~fresh;  // cells below the last new one
     uint8_t* const sc = p.scales + (size_t)(slot >> 4) * p.block_scales + p.layer_scale + h;
     const uint32_t had_byte = *sc;
-    const SRC* const src = reinterpret_cast<const SRC*>(p.qkv) + (size_t)(p.H + h) * DH + lane * N;
-    float* const mine = stage + lane * N;
-    float amax = 0.f;
-    constexpr int U = 4;  // rows loaded together
+    const SRC* const src = reinterpret_cast<const SRC*>(p.qkv) + (size_t)(p.H + h) * DH + d;
+    float* const mine = stage + sub * DH + d;
+    const bool norm = key && p.k_gain, turn = key && p.rope;
+    float amax = 0.f, gain[8];
+    if (norm) load8(p.k_gain + d, gain);
+    constexpr int U = 2;  // steps whose loads go out together
 #pragma unroll 1
-    for (int i0 = 0; i0 < run; i0 += U) {
-        float v[U][N];
-        int row[U];
+    for (int i0 = 0; i0 < run; i0 += U * RPW) {
+        float v[U][8], cs[U][8];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            row[u] = __shfl_sync(0xffffffffu, row_i, (i0 + u) & 31);
-            if (i0 + u < run) load_row<N>(src + (size_t)row[u] * p.qkv_stride, v[u]);
+            const int i = i0 + u * RPW + sub, row = __shfl_sync(0xffffffffu, row_i, i & 31);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[u][k] = cs[u][k] = 0.f;
+            if (i < run) {
+                load8(src + (size_t)row * p.qkv_stride, v[u]);
+                if (turn) load8(reinterpret_cast<const float*>(p.rope + (size_t)row * (DH / 2)) + d, cs[u]);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (i0 + u < run) {
-                if (key) norm_rotate<DH, N>(p, p.k_gain, row[u], lane, v[u]);
+            const int i = i0 + u * RPW + sub;
+            norm_rotate<DH>(norm, turn, p.eps, gain, cs[u], v[u]);
+            if (i < run) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float a = fabsf(v[u][j]);
+                for (int k = 0; k < 8; ++k) {
+                    const float a = fabsf(v[u][k]);
                     amax = a <= 3.402823466e38f ? fmaxf(amax, a) : amax;  // finite values only
                 }
-                store_row<N>(mine + (i0 + u) * DH, v[u]);
+                store8(mine + (i0 + u * RPW) * DH, v[u]);
             }
         }
     }
@@ -220,21 +228,16 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int t, int s
     if (lane == 0) *sc = (uint8_t)(e + KV8_BIAS);
     const float f = exp2_int(-e);
 #pragma unroll 2
-    for (int i = 0; i < run; ++i) {
-        float v[N];
-        load_row<N>(mine + i * DH, v);  // (this lane's own values)
-        uint8_t* const o = cells + (size_t)__shfl_sync(0xffffffffu, off_i, i) * DH + lane * N;
-        const uint32_t a = e4m3x2_from(v[0] * f, v[1] * f);
-        if constexpr (N == 2) {
-            *reinterpret_cast<uint16_t*>(o) = (uint16_t)a;
-        } else {
-            const uint32_t b = a | (e4m3x2_from(v[2] * f, v[3] * f) << 16);
-            if constexpr (N == 4) {
-                *reinterpret_cast<uint32_t*>(o) = b;
-            } else {
-                const uint32_t c = e4m3x2_from(v[4] * f, v[5] * f) | (e4m3x2_from(v[6] * f, v[7] * f) << 16);
-                *reinterpret_cast<uint2*>(o) = make_uint2(b, c);
-            }
+    for (int i0 = 0; i0 < run; i0 += RPW) {
+        const int i = i0 + sub, off = __shfl_sync(0xffffffffu, off_i, i & 31);
+        if (i < run) {
+            float v[8];
+            load8(mine + i0 * DH, v);  // (this lane's own values)
+            uint32_t w[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                w[k] = e4m3x2_from(v[4 * k] * f, v[4 * k + 1] * f) | (e4m3x2_from(v[4 * k + 2] * f, v[4 * k + 3] * f) << 16);
+            *reinterpret_cast<uint2*>(cells + (size_t)off * DH + d) = make_uint2(w[0], w[1]);
         }
     }
 }
@@ -242,17 +245,16 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int t, int s
 // The first row_blocks CTAs take single rows, the others (e4m3) blocks: a warp
 // looks at `tile` consecutive rows (at most 16) for those that begin a block.
 // Bytes bound it: every row is read once.  What the shape is after is loads in
-// flight: ROWS rows a warp where there are rows enough (4: 8192 tokens), one
-// where there are not (decode), and values in shared memory rather than
-// registers so that 28 warps share an SM.
-template <typename SRC, typename DST, bool E4M3, int DH, int ROWS>
+// flight and few instructions a byte: 16 bytes of bf16 a lane, STEPS rows of
+// loads a warp where there are rows enough, one where there are not (decode).
+template <typename SRC, typename DST, bool E4M3, int DH, int STEPS>
 __global__ void __launch_bounds__(128, DH == 256 ? 3 : 7) kv_append_kernel(const __grid_constant__ AppendParams p, unsigned row_blocks, int tile) {
     extern __shared__ __align__(16) float append_stage[];
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x < row_blocks) {
-        append_rows<SRC, DST, E4M3, DH, ROWS>(p, ((long long)blockIdx.x * 4 + warp) * ROWS, lane);
+        append_rows<SRC, DST, E4M3, DH, STEPS>(p, (long long)blockIdx.x * 4 + warp, lane);
         return;
     }
     if constexpr (E4M3) {
@@ -282,11 +284,13 @@ __global__ void __launch_bounds__(128, DH == 256 ? 3 : 7) kv_append_kernel(const
 
 template <typename SRC, typename DST, bool E4M3, int DH>
 static cudaError_t launch_append_dh(cudaStream_t st, bool pdl, int sms, const AppendParams& p) {
-    const long long rows = (long long)p.T * (E4M3 ? p.H : p.H + 2 * p.G);
+    constexpr int RPW = 256 / DH, STEPS = 4;
+    const int heads = E4M3 ? p.H : p.H + 2 * p.G;
     const long long warps = (long long)sms * 28;
-    const int per_warp = rows >= 4 * warps ? 4 : 1;
-    const unsigned row_blocks = (unsigned)((rows + 4 * per_warp - 1) / (4 * per_warp));
-    // rows a warp looks through: 16 once that still fills the device
+    const auto tasks = [&](int steps) { return (long long)p.T * ((heads + steps * RPW - 1) / (steps * RPW)); };
+    const int steps = tasks(STEPS) >= warps ? STEPS : 1;  // (several rows a warp once that still fills the device)
+    const unsigned row_blocks = (unsigned)((tasks(steps) + 3) / 4);
+    // rows a warp looks through for blocks: by the same rule
     int tile = 1;
     while (tile < 16 && (long long)p.T * 2 * p.G >= 2 * tile * warps) tile *= 2;
     const unsigned blocks = E4M3 ? (unsigned)((((long long)p.T + tile - 1) / tile * 2 * p.G + 3) / 4) : 0;
@@ -297,14 +301,14 @@ static cudaError_t launch_append_dh(cudaStream_t st, bool pdl, int sms, const Ap
         if (const cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
         const uint64_t bit = 1ull << (dev & 63);
         if (!(ready.load(std::memory_order_acquire) & bit)) {
-            for (auto* f : {kv_append_kernel<SRC, DST, E4M3, DH, 4>, kv_append_kernel<SRC, DST, E4M3, DH, 1>})
+            for (auto* f : {kv_append_kernel<SRC, DST, E4M3, DH, STEPS>, kv_append_kernel<SRC, DST, E4M3, DH, 1>})
                 if (const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); e != cudaSuccess)
                     return e;
             ready.fetch_or(bit, std::memory_order_release);
         }
     }
-    if (per_warp == 4)
-        return launch_on(st, pdl, kv_append_kernel<SRC, DST, E4M3, DH, 4>, row_blocks + blocks, 128, smem, p, row_blocks, tile);
+    if (steps > 1)
+        return launch_on(st, pdl, kv_append_kernel<SRC, DST, E4M3, DH, STEPS>, row_blocks + blocks, 128, smem, p, row_blocks, tile);
     return launch_on(st, pdl, kv_append_kernel<SRC, DST, E4M3, DH, 1>, row_blocks + blocks, 128, smem, p, row_blocks, tile);
 }
 
