@@ -97,6 +97,8 @@ typedef struct yk_model_config {
 #define YK_T_NORM2      9  /* [d]                  rmsGamma2                     */
 #define YK_T_FINAL_NORM 10 /* [d]                  finalNormGamma                */
 #define YK_T_LM_HEAD    11 /* [vocab x d]          LMHead.projection             */
+#define YK_T_QNORM      12 /* [head_dim]           per-head query norm (yk_model_enable_qk_norm) */
+#define YK_T_KNORM      13 /* [head_dim]           per-head key norm             */
 
 #define YK_LAYOUT_OUT_IN 0 /* [out x in], this module's layout                     */
 #define YK_LAYOUT_IN_OUT 1 /* [in x out], the reference's LinearLayer layout
@@ -137,6 +139,11 @@ yk_status yk_model_create(yk_engine* e, const yk_model_config* cfg, uint64_t see
 void      yk_model_destroy(yk_model* m);
 yk_status yk_model_get_config(const yk_model* m, yk_model_config* out);
 yk_status yk_model_tensor_shape(const yk_model* m, int32_t tensor, int64_t* rows, int64_t* cols);
+/* Per-head norms of queries and keys, x / sqrt(mean(x^2) + rms_eps) * gain before
+ * the rotation (checkpoints with q_norm / k_norm; the reference has none).  Adds
+ * YK_T_QNORM and YK_T_KNORM to every layer, gains 1.  Not with ref_compat
+ * (YK_ERR_UNSUPPORTED); calling it again changes nothing. */
+yk_status yk_model_enable_qk_norm(yk_model* m);
 /* Upload one logical tensor from fp32 host memory (converted to the model dtype). */
 yk_status yk_model_set_tensor(yk_model* m, int32_t tensor, int32_t layer, const float* host,
                               int32_t layout);
@@ -182,7 +189,8 @@ yk_status yk_model_load_tensor(yk_model* m, int32_t tensor, int32_t layer, const
  * Hugging Face Llama / Gemma names (model.embed_tokens.weight,
  * model.layers.N.self_attn.{q,k,v,o}_proj.weight, mlp.{gate,up,down}_proj.weight,
  * input_layernorm.weight, post_attention_layernorm.weight, model.norm.weight,
- * lm_head.weight -- absent: tied to the embedding).  norm_offset is added to
+ * lm_head.weight -- absent: tied to the embedding; self_attn.{q,k}_norm.weight,
+ * wanted of a model with per-head norms and unsupported by one without).  norm_offset is added to
  * every norm gain (1 for checkpoints that store gain - 1).  A missing tensor, a
  * shape mismatch or a tensor in two files is YK_ERR_ARG; an unknown tensor of a
  * decoder layer (a layer kind this module lacks) is YK_ERR_UNSUPPORTED. */
@@ -213,6 +221,14 @@ yk_status yk_kv_pool_create(yk_engine* e, const yk_model_config* cfg, int32_t nu
 #define YK_POOL_WINDOWED_LAYERS 2
 yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks, int32_t layers,
                                    yk_kv_pool** out);
+/* A pool of 8-bit cells (YK_KV_E4M3 below: e4m3 with one scale byte for each
+ * block, layer, K|V and kv head) for a model of cfg's shape, bf16 or fp32: half
+ * (a quarter) of the memory of yk_kv_pool_create's, and of the bytes attention
+ * reads.  Every forward call takes it in the other's place (split pools: both of
+ * them); the keys and values of a step are stored by yk_kv_append's kernel and
+ * read by yk_attention_e4m3's.  Not for ref_compat models. */
+yk_status yk_kv_pool_create_e4m3(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks, int32_t layers,
+                                 yk_kv_pool** out);
 void      yk_kv_pool_destroy(yk_kv_pool* p);
 int32_t   yk_kv_pool_num_blocks(const yk_kv_pool* p);
 /* Fills every slot with N(0, std) values (synthetic context for benchmarks). */
@@ -286,6 +302,10 @@ typedef struct yk_kv_pages {
     int32_t  n_kv_heads;
     int32_t  head_dim;
 } yk_kv_pages;
+/* The memory of a pool of the module, for the calls below (valid until
+ * yk_kv_pool_destroy; layer l of a YK_POOL_GLOBAL_LAYERS / WINDOWED_LAYERS pool is
+ * the l-th of its kind).  The engine's own steps use it on the engine's stream. */
+yk_status yk_kv_pool_pages(yk_kv_pool* p, yk_kv_pages* out);
 
 /* Between the QKV product and attention, in one pass over the projections:
  * row t of qkv holds n_heads query heads, then n_kv_heads key heads, then

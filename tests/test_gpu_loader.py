@@ -234,3 +234,41 @@ def test_safetensors_checkpoint_errors(engine, tmp_path):
     finally:
         pool.close()
         m.close()
+
+
+@pytest.mark.parametrize("flags", [0, abi.LOAD_ROPE_HALF])
+def test_safetensors_per_head_norms(engine, tmp_path, flags):
+    """q_norm / k_norm of a model with per-head norms: bit-exact, a gain following its head's rows out of
+    rotate-half order; missing ones are an error, and so is their presence for a model without."""
+    rng = np.random.default_rng(6)
+    dh, L = TINY["head_dim"], TINY["n_layers"]
+    norms = {f"model.layers.{l}.self_attn.{n}_norm.weight": (dh,) for l in range(L) for n in "qk"}
+    (tmp_path / "with").mkdir()
+    (tmp_path / "without").mkdir()
+    paths, arrays = _hf_checkpoint(rng, TINY, tmp_path / "with", extra=norms)
+    bare, _ = _hf_checkpoint(rng, TINY, tmp_path / "without")
+    m, pool = gpu_model(engine, TINY, abi.DTYPE_BF16, seed=7, num_blocks=4)
+    files, bare = [abi.SafeTensors(p) for p in paths], [abi.SafeTensors(p) for p in bare]
+    try:
+        with pytest.raises(abi.YKError) as ei:
+            m.load_safetensors(files, flags=flags)
+        assert ei.value.status == 7 and "_norm" in str(ei.value)
+        m.enable_qk_norm()
+        with pytest.raises(abi.YKError) as ei:
+            m.load_safetensors(bare, flags=flags)
+        assert ei.value.status == 1 and "lacks tensor" in str(ei.value)
+        assert m.load_safetensors(files, flags=flags) == 3 + 11 * L
+        for l in range(L):
+            for t, n in ((abi.T_QNORM, "q"), (abi.T_KNORM, "k")):
+                want = _f32(arrays[f"model.layers.{l}.self_attn.{n}_norm.weight"])
+                if flags:
+                    want = unpermute_rope_half(want[:, None], dh)[:, 0]
+                assert (m.get(t, l).ravel() == want).all(), (l, n)
+        assert m.load_safetensors(files, norm_offset=1.0) == 3 + 11 * L
+        assert np.array_equal(m.get(abi.T_KNORM, 1).ravel(),
+                              _f32(arrays["model.layers.1.self_attn.k_norm.weight"]) + np.float32(1.0))
+    finally:
+        for f in files + bare:
+            f.close()
+        pool.close()
+        m.close()

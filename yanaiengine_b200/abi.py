@@ -21,7 +21,7 @@ LOAD_ROPE_HALF = 1
 ACT_SILU, ACT_GELU_TANH = 0, 1
 BLOCK_SIZE = 16
 (T_EMBED, T_WQ, T_WK, T_WV, T_WO, T_WGATE, T_WUP, T_WDOWN, T_NORM1, T_NORM2, T_FINAL_NORM,
- T_LM_HEAD) = range(12)
+ T_LM_HEAD, T_QNORM, T_KNORM) = range(14)
 LAYOUT_OUT_IN, LAYOUT_IN_OUT = 0, 1
 KV_F32, KV_BF16, KV_E4M3 = 0, 1, 2
 
@@ -146,6 +146,9 @@ _PROTOS = {
     "yk_tp_allgather_u32": (C.c_int32, [_P, _U32P, C.c_int32, _U32P]),
     "yk_spec_verify_logits_noalloc": (C.c_int32, [C.c_int32, _P, _P, _P, _P, _P, C.c_int32, C.c_int32, C.c_int32,
                                                   C.c_float, C.c_uint64, C.c_uint32, _P, _P]),
+    "yk_kv_pool_create_e4m3": (C.c_int32, [_P, C.POINTER(ModelConfig), C.c_int32, C.c_int32, C.POINTER(_P)]),
+    "yk_kv_pool_pages": (C.c_int32, [_P, C.POINTER(KVPages)]),
+    "yk_model_enable_qk_norm": (C.c_int32, [_P]),
     "yk_kv_append": (C.c_int32, [C.c_int32, _P, _P]),
     "yk_attention_e4m3": (C.c_int32, [C.c_int32, _P, _P]),
     "yk_attention_e4m3_workspace": (C.c_int32, [C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
@@ -600,6 +603,10 @@ class Model:
             check(lib().yk_model_get_config(self.h, C.byref(shard)))
             self.cfg = shard  # the shard's heads / FFN: the config its KV pool is created with
 
+    def enable_qk_norm(self):
+        """Per-head norms of queries and keys (T_QNORM, T_KNORM; gains 1)."""
+        check(lib().yk_model_enable_qk_norm(self.h))
+
     def shape(self, t: int) -> tuple[int, int]:
         r, c = C.c_int64(), C.c_int64()
         check(lib().yk_model_tensor_shape(self.h, t, C.byref(r), C.byref(c)))
@@ -687,11 +694,19 @@ POOL_ALL_LAYERS, POOL_GLOBAL_LAYERS, POOL_WINDOWED_LAYERS = 0, 1, 2
 
 
 class KVPool:
-    def __init__(self, engine: Engine, cfg: ModelConfig, num_blocks: int, layers: int = POOL_ALL_LAYERS):
-        """layers: POOL_ALL_LAYERS, or one kind of layer (yk_kv_pool_create_layers)."""
+    def __init__(self, engine: Engine, cfg: ModelConfig, num_blocks: int, layers: int = POOL_ALL_LAYERS,
+                 e4m3: bool = False):
+        """layers: POOL_ALL_LAYERS, or one kind of layer (yk_kv_pool_create_layers); e4m3: 8-bit cells."""
         self.cfg = cfg
         self.h = _P()
-        check(lib().yk_kv_pool_create_layers(engine.h, C.byref(cfg), num_blocks, layers, C.byref(self.h)))
+        create = lib().yk_kv_pool_create_e4m3 if e4m3 else lib().yk_kv_pool_create_layers
+        check(create(engine.h, C.byref(cfg), num_blocks, layers, C.byref(self.h)))
+
+    def pages(self) -> KVPages:
+        """The pool's device memory (yk_kv_pool_pages)."""
+        p = KVPages()
+        check(lib().yk_kv_pool_pages(self.h, C.byref(p)))
+        return p
 
     def fill_random(self, seed: int, std: float):
         check(lib().yk_kv_pool_fill_random(self.h, seed, std))

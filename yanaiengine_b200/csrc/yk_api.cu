@@ -10,6 +10,7 @@
 
 #include "yk_common.cuh"
 #include "yk_internal.h"
+#include "yk_kvcache.cuh"
 
 static thread_local std::string g_last_error;
 void yk_set_error(const std::string& msg) { g_last_error = msg; }
@@ -236,6 +237,13 @@ static float host_from_bf16(uint16_t b) {
     return f;
 }
 
+static float host_e4m3(uint8_t c) {  // sign, 4 bits of exponent (bias 7), 3 of mantissa; no infinities
+    const int e = (c >> 3) & 15, m = c & 7;
+    if ((c & 127) == 127) return std::nanf("");
+    const float v = e == 0 ? std::ldexp((float)m, -9) : std::ldexp(8.0f + m, e - 10);
+    return c & 128 ? -v : v;
+}
+
 static yk_status dalloc(yk_model* m, void** p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, std::max<size_t>(bytes, 256));
     if (e != cudaSuccess) {
@@ -402,7 +410,30 @@ extern "C" void yk_model_destroy(yk_model* m) {
     if (m->gemm_stamps) cudaFree(m->gemm_stamps);
     if (m->chain_bar) cudaFree(m->chain_bar);
     if (m->gemm_counters) cudaFree(m->gemm_counters);
+    if (m->attn8_ws) cudaFree(m->attn8_ws);
     delete m;
+}
+
+extern "C" yk_status yk_model_enable_qk_norm(yk_model* m) {
+    YK_ARG(m, "null handle");
+    if (m->cfg.ref_compat) {
+        yk_set_error("unsupported: per-head norms of a ref_compat model");
+        return YK_ERR_UNSUPPORTED;
+    }
+    if (m->qk_norm) return YK_OK;
+    YK_CHECK_CUDA(cudaSetDevice(m->e->device));
+    const size_t dh = m->cfg.head_dim;
+    float* g = nullptr;  // one allocation for all layers
+    YK_TRY(dalloc(m, (void**)&g, (size_t)2 * m->cfg.n_layers * dh * 4));
+    YK_TRY(yk::launch_init(m->e, g, (size_t)2 * m->cfg.n_layers * dh, YK_DTYPE_F32, 0, 0, 1.0f, true));
+    YK_CHECK_CUDA(cudaStreamSynchronize(m->e->stream));
+    for (auto& L : m->layers) {
+        L.qn = g;
+        L.kn = g + dh;
+        g += 2 * dh;
+    }
+    m->qk_norm = true;
+    return YK_OK;
 }
 
 extern "C" yk_status yk_model_get_config(const yk_model* m, yk_model_config* out) {
@@ -415,8 +446,9 @@ yk_status yk::locate_tensor(const yk_model* m, int32_t t, int32_t layer, TensorL
     const auto& c = m->cfg;
     const size_t d = c.d_model, dh = c.head_dim, qd = (size_t)c.n_heads * dh, kvd = (size_t)c.n_kv_heads * dh;
     const size_t es = m->esize;
-    const bool per_layer = t >= YK_T_WQ && t <= YK_T_NORM2;
-    YK_ARG(t >= 0 && t <= YK_T_LM_HEAD, "tensor id");
+    const bool per_layer = (t >= YK_T_WQ && t <= YK_T_NORM2) || t == YK_T_QNORM || t == YK_T_KNORM;
+    YK_ARG(t >= 0 && t <= YK_T_KNORM, "tensor id");
+    YK_ARG(m->qk_norm || (t != YK_T_QNORM && t != YK_T_KNORM), "the model has no per-head norms (yk_model_enable_qk_norm)");
     if (per_layer) YK_ARG(layer >= 0 && layer < c.n_layers, "layer index");
     const LayerWeights* W = per_layer ? &m->layers[layer] : nullptr;
     switch (t) {
@@ -431,6 +463,8 @@ yk_status yk::locate_tensor(const yk_model* m, int32_t t, int32_t layer, TensorL
         case YK_T_NORM1: *L = {(uint8_t*)W->n1, 0, 1, 1, d, 4}; break;
         case YK_T_NORM2: *L = {(uint8_t*)W->n2, 0, 1, 1, d, 4}; break;
         case YK_T_FINAL_NORM: *L = {(uint8_t*)m->final_norm, 0, 1, 1, d, 4}; break;
+        case YK_T_QNORM: *L = {(uint8_t*)W->qn, 0, 1, 1, dh, 4}; break;
+        case YK_T_KNORM: *L = {(uint8_t*)W->kn, 0, 1, 1, dh, 4}; break;
         case YK_T_LM_HEAD: *L = {(uint8_t*)m->lm_head, 0, 1, (size_t)c.vocab_size, d, es}; break;
     }
     return YK_OK;
@@ -488,8 +522,8 @@ extern "C" yk_status yk_model_get_tensor(yk_model* m, int32_t t, int32_t layer, 
 // ---------------------------------------------------------------------------
 // KV pool
 // ---------------------------------------------------------------------------
-extern "C" yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks,
-                                              int32_t layers, yk_kv_pool** out) {
+static yk_status create_pool(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks, int32_t layers, bool e4m3,
+                             yk_kv_pool** out) {
     YK_ARG(e && out, "null handle");
     *out = nullptr;
     YK_TRY(validate_cfg(cfg));
@@ -505,7 +539,8 @@ extern "C" yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_confi
     p->num_blocks = num_blocks;
     p->kind = layers;
     p->n_pool_layers = n_pool_layers;
-    p->esize = cfg->dtype == YK_DTYPE_BF16 ? 2 : 4;
+    p->esize = e4m3 ? 1 : cfg->dtype == YK_DTYPE_BF16 ? 2 : 4;
+    p->cells = e4m3 ? YK_KV_E4M3 : cfg->dtype == YK_DTYPE_BF16 ? YK_KV_BF16 : YK_KV_F32;
     p->layer_elems = (size_t)2 * cfg->n_kv_heads * YK_BLOCK_SIZE * cfg->head_dim;
     p->block_elems = p->layer_elems * n_pool_layers;
     const size_t bytes = p->block_elems * num_blocks * p->esize;
@@ -522,7 +557,19 @@ extern "C" yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_confi
         yk_set_error(std::string("KV pool memset: ") + cudaGetErrorString(err));
         return YK_ERR_CUDA;
     }
-    if (cfg->dtype == YK_DTYPE_BF16) {
+    if (e4m3) {
+        // scale bytes: the smallest exponent, so that a block's first values set theirs
+        const size_t n = (size_t)num_blocks * n_pool_layers * 2 * cfg->n_kv_heads;
+        err = cudaMalloc(&p->scales, n);
+        if (err == cudaSuccess) err = cudaMemset(p->scales, yk::KV8_BIAS + yk::KV8_EMIN, n);
+        if (err != cudaSuccess) {
+            if (p->scales) cudaFree(p->scales);
+            cudaFree(p->data);
+            delete p;
+            yk_set_error("KV pool scales (" + std::to_string(n) + " bytes): " + cudaGetErrorString(err));
+            return err == cudaErrorMemoryAllocation ? YK_ERR_OOM : YK_ERR_CUDA;
+        }
+    } else if (cfg->dtype == YK_DTYPE_BF16) {
         const yk_status s = yk::make_pool_map(e, p);
         if (s != YK_OK) {
             cudaFree(p->data);
@@ -531,6 +578,27 @@ extern "C" yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_confi
         }
     }
     *out = p;
+    return YK_OK;
+}
+
+extern "C" yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks,
+                                              int32_t layers, yk_kv_pool** out) {
+    return create_pool(e, cfg, num_blocks, layers, false, out);
+}
+
+extern "C" yk_status yk_kv_pool_create_e4m3(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks, int32_t layers,
+                                            yk_kv_pool** out) {
+    if (out) *out = nullptr;
+    if (cfg && cfg->ref_compat) {
+        yk_set_error("unsupported: an e4m3 KV pool for a ref_compat model");
+        return YK_ERR_UNSUPPORTED;
+    }
+    return create_pool(e, cfg, num_blocks, layers, true, out);
+}
+
+extern "C" yk_status yk_kv_pool_pages(yk_kv_pool* p, yk_kv_pages* out) {
+    YK_ARG(p && out, "null handle");
+    *out = yk::pool_pages(p);
     return YK_OK;
 }
 
@@ -543,6 +611,7 @@ extern "C" void yk_kv_pool_destroy(yk_kv_pool* p) {
     cudaSetDevice(p->e->device);
     cudaStreamSynchronize(p->e->stream);
     cudaFree(p->data);
+    if (p->scales) cudaFree(p->scales);
     delete p;
 }
 
@@ -551,6 +620,11 @@ extern "C" int32_t yk_kv_pool_num_blocks(const yk_kv_pool* p) { return p ? p->nu
 extern "C" yk_status yk_kv_pool_fill_random(yk_kv_pool* p, uint64_t seed, float std) {
     YK_ARG(p, "null handle");
     YK_CHECK_CUDA(cudaSetDevice(p->e->device));
+    if (p->cells == YK_KV_E4M3) {
+        YK_TRY(yk::launch_fill_e4m3(p, seed, std));
+        YK_CHECK_CUDA(cudaStreamSynchronize(p->e->stream));
+        return YK_OK;
+    }
     YK_TRY(yk::launch_init(p->e, p->data, p->block_elems * p->num_blocks, p->cfg.dtype, seed, 0x4B56u, std, false));
     YK_CHECK_CUDA(cudaStreamSynchronize(p->e->stream));
     return YK_OK;
@@ -565,12 +639,23 @@ extern "C" yk_status yk_kv_pool_read_page(yk_kv_pool* p, int32_t block, int32_t 
     yk_engine* e = p->e;
     YK_CHECK_CUDA(cudaSetDevice(e->device));
     const size_t n = (size_t)p->cfg.n_kv_heads * YK_BLOCK_SIZE * p->cfg.head_dim;
-    YK_TRY(e->ensure_pinned(n * p->esize));
+    const int G = p->cfg.n_kv_heads;
+    YK_TRY(e->ensure_pinned(n * p->esize + G));
     YK_CHECK_CUDA(cudaStreamSynchronize(e->stream));
+    if (p->cells == YK_KV_E4M3)
+        YK_CHECK_CUDA(cudaMemcpyAsync(e->pinned + n, p->scales + (((size_t)block * p->n_pool_layers + pl) * 2 + kv) * G, G,
+                                      cudaMemcpyDeviceToHost, e->stream));
     const uint8_t* src = (const uint8_t*)p->data + ((size_t)block * p->block_elems + (size_t)pl * p->layer_elems +
                                                     (size_t)kv * n) * p->esize;
     YK_CHECK_CUDA(cudaMemcpyAsync(e->pinned, src, n * p->esize, cudaMemcpyDeviceToHost, e->stream));
     YK_CHECK_CUDA(cudaStreamSynchronize(e->stream));
+    if (p->cells == YK_KV_E4M3) {
+        const size_t per = n / G;  // values of one head
+        for (int g = 0; g < G; ++g)
+            for (size_t i = 0; i < per; ++i)
+                host[g * per + i] = std::ldexp(host_e4m3(e->pinned[g * per + i]), yk::kv8_exponent(e->pinned[n + g]));
+        return YK_OK;
+    }
     for (size_t i = 0; i < n; ++i)
         host[i] = p->esize == 2 ? host_from_bf16(((uint16_t*)e->pinned)[i]) : ((float*)e->pinned)[i];
     return YK_OK;
@@ -588,6 +673,67 @@ struct WindowedPool {
     const int32_t* tables = nullptr;
     int32_t max_blocks = 0;
 };
+
+// The step's raw projections: queries to m->q, keys and values to the pool.
+static yk_status append_raw(yk_model* m, const LayerWeights& L, yk_kv_pool* pool, int pool_layer, int T, const int32_t* slots) {
+    const auto& c = m->cfg;
+    yk_engine* e = m->e;
+    yk_kv_append_args a{};
+    a.pages = yk::pool_pages(pool);
+    a.layer = pool_layer;
+    a.T = T;
+    a.n_heads = c.n_heads;
+    a.src_dtype = YK_DTYPE_F32;
+    a.q_dtype = c.dtype;
+    a.eps = c.rms_eps;
+    a.qkv = m->qkv_raw;
+    a.qkv_stride = (int64_t)(c.n_heads + 2 * c.n_kv_heads) * c.head_dim;
+    a.q_out = m->q;
+    a.q_stride = (int64_t)c.n_heads * c.head_dim;
+    a.slots = slots;
+    a.rope = reinterpret_cast<const float*>(m->rope_tab);
+    a.q_gain = L.qn;
+    a.k_gain = L.kn;
+    a.err = e->d_err;
+    const double rows = (double)T * c.head_dim;
+    ProfScope prof(e, YK_PROF_OTHER, rows * ((c.n_heads + 2.0 * c.n_kv_heads) * 4 + c.n_heads * (double)m->esize +
+                                             2.0 * c.n_kv_heads * (double)pool->esize), 0.0);
+    YK_TRY(yk::kv_append_check(a));
+    YK_TRY(yk::kv_append_launch(e->stream, e->pdl && !e->profiling, e->num_sms, a));
+    e->launches++;
+    return YK_OK;
+}
+
+static yk_status attend_e4m3(yk_model* m, yk_kv_pool* pool, int pool_layer, int T, int B, const int32_t* bt, int32_t max_blocks,
+                             int32_t most_new, int32_t window, double kv_bytes) {
+    const auto& c = m->cfg;
+    yk_engine* e = m->e;
+    yk_attention_e4m3_args a{};
+    a.pages = yk::pool_pages(pool);
+    a.layer = pool_layer;
+    a.T = T;
+    a.B = B;
+    a.n_heads = c.n_heads;
+    a.dtype = c.dtype;
+    a.max_blocks = max_blocks;
+    a.max_new = most_new;
+    a.window = window;
+    a.cap = c.attn_cap;
+    a.q = m->q;
+    a.out = m->att;
+    a.q_stride = a.out_stride = (int64_t)c.n_heads * c.head_dim;
+    a.q_starts = m->cur.q_starts;
+    a.context_lens = m->cur.ctx;
+    a.block_tables = bt;
+    a.workspace = m->attn8_ws;
+    a.workspace_bytes = m->attn8_ws_bytes;
+    a.err = e->d_err;
+    ProfScope prof(e, YK_PROF_ATTN, kv_bytes + 2.0 * T * c.n_heads * c.head_dim * (double)m->esize, 0.0);
+    YK_TRY(yk::attention_e4m3_check(a));
+    YK_TRY(yk::attention_e4m3_launch(e->stream, e->pdl && !e->profiling, e->num_sms, a));
+    e->launches++;
+    return YK_OK;
+}
 
 static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tokens, int32_t T,
                               const uint32_t* q_starts, const uint32_t* ctx, int32_t B, const int32_t* block_tables,
@@ -613,6 +759,15 @@ static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tok
     YK_ARG(pool->cfg.n_layers == c.n_layers && pool->cfg.n_kv_heads == c.n_kv_heads &&
                pool->cfg.head_dim == c.head_dim && pool->cfg.dtype == c.dtype,
            "pool shape does not match the model");
+    const bool e4 = pool->cells == YK_KV_E4M3;
+    YK_ARG(!wpool || (wpool->cells == YK_KV_E4M3) == e4, "split pools: both with 8-bit cells, or neither");
+    // queries and keys normed per head, or 8-bit cells: the projections go to memory
+    // as they are, and yk_kv_append's kernel takes them from there
+    const bool raw_qkv = e4 || m->qk_norm;
+    if (raw_qkv && c.ref_compat) {
+        yk_set_error("unsupported: ref_compat with per-head norms or an e4m3 pool");
+        return YK_ERR_UNSUPPORTED;
+    }
     YK_ARG(T > 0 && T <= c.max_tokens, "T must be in [1, max_tokens]");
     YK_ARG(B > 0 && B <= c.max_seqs, "B must be in [1, max_seqs]");
     YK_ARG(max_blocks > 0 && last_n >= 0, "max_blocks / last_n");
@@ -648,7 +803,17 @@ static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tok
     static thread_local std::vector<int32_t> it_g, cb_g, it_w, cb_w;
     int slots_g = 0, slots_w = 0;
     it_g.clear(); cb_g.clear(); it_w.clear(); cb_w.clear();
-    if (c.dtype == YK_DTYPE_BF16) {
+    int most_new = 0;
+    for (int b = 0; b < B; ++b) most_new = std::max(most_new, (int)(q_starts[b + 1] - q_starts[b]));
+    if (raw_qkv && !m->qkv_raw)
+        YK_TRY(dalloc(m, (void**)&m->qkv_raw, (size_t)c.max_tokens * (c.n_heads + 2 * c.n_kv_heads) * c.head_dim * 4));
+    if (e4 && !m->attn8_ws) {
+        const size_t n = yk::attention_e4m3_ws_bytes(e->num_sms, c.head_dim);
+        YK_CHECK_CUDA(cudaMalloc(&m->attn8_ws, n));
+        YK_CHECK_CUDA(cudaMemsetAsync(m->attn8_ws, 0, n, e->stream));  // (its first user is on the same stream)
+        m->attn8_ws_bytes = n;
+    }
+    if (c.dtype == YK_DTYPE_BF16 && !e4) {
         yk::plan_attention(c, e->num_sms, e->attn_waves, e->attn_balanced, q_starts, ctx, B, false, it_g, cb_g,
                            &slots_g);
         if (c.window > 0)
@@ -802,7 +967,7 @@ static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tok
         kv_full += (double)ctx[b];
         kv_win += c.window > 0 ? std::min((double)ctx[b], (double)c.window + n - 1) : (double)ctx[b];
     }
-    const double kv_tok_bytes = 2.0 * kvd * (double)m->esize;
+    const double kv_tok_bytes = 2.0 * kvd * (double)pool->esize;
     // Tensor parallel: o_proj / down_proj write partials (bf16, or fp32 with
     // YK_TP_PAYLOAD=f32) that are summed across the group; the sum is added to the
     // residual stream by the next RMSNorm.
@@ -867,10 +1032,22 @@ static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tok
         eq.block_elems = (long long)lpool->block_elems;
         eq.layer_off = (long long)pl * (long long)lpool->layer_elems;
         eq.pool_blocks = lpool->num_blocks;
-        norm_in(eq);
-        YK_TRY(gemm_run(m, L.wqkv, &L.tm_qkv, m->xn, qd + 2 * kvd, d, T, eq));
-        YK_TRY(attention_run(m, lpool, l, pl, in_w ? m->cur.wbt : m->cur.bt, T, B, in_w ? wp.max_blocks : max_blocks,
-                             (windowed ? kv_win : kv_full) * kv_tok_bytes));
+        const int32_t* const l_bt = in_w ? m->cur.wbt : m->cur.bt;
+        const int32_t l_max_blocks = in_w ? wp.max_blocks : max_blocks;
+        const double l_kv_bytes = (windowed ? kv_win : kv_full) * kv_tok_bytes;
+        if (raw_qkv) {
+            EpiParams ew;
+            ew.kind = EPI_STORE;
+            ew.out = m->qkv_raw;
+            norm_in(ew);
+            YK_TRY(gemm_run(m, L.wqkv, &L.tm_qkv, m->xn, qd + 2 * kvd, d, T, ew));
+            YK_TRY(append_raw(m, L, lpool, pl, T, eq.slot));
+        } else {
+            norm_in(eq);
+            YK_TRY(gemm_run(m, L.wqkv, &L.tm_qkv, m->xn, qd + 2 * kvd, d, T, eq));
+        }
+        if (e4) YK_TRY(attend_e4m3(m, lpool, pl, T, B, l_bt, l_max_blocks, most_new, windowed ? c.window : 0, l_kv_bytes));
+        else YK_TRY(attention_run(m, lpool, l, pl, l_bt, T, B, l_max_blocks, l_kv_bytes));
         EpiParams er;
         er.kind = EPI_RESID;
         er.ref_compat = c.ref_compat;

@@ -1012,12 +1012,12 @@ static yk_status launch_tc(const cudaLaunchConfig_t& cfg, const CUtensorMap* tmW
     if (!attr) {
         YK_CHECK_CUDA(cudaFuncSetAttribute(gemm_tc_kernel<KIND, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                            TC_SMEM_BUDGET + 16384 + TC_SMEM_TAIL));
-        if constexpr (KIND == EPI_QKV || KIND == EPI_RESID || KIND == EPI_GLU)
+        if constexpr (KIND == EPI_QKV || KIND == EPI_RESID || KIND == EPI_GLU || KIND == EPI_STORE)
             YK_CHECK_CUDA(cudaFuncSetAttribute(gemm_tc_kernel<KIND, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                TC_SMEM_BUDGET + 16384 + TC_SMEM_TAIL));
         attr = true;
     }
-    if constexpr (KIND == EPI_QKV || KIND == EPI_RESID || KIND == EPI_GLU) {
+    if constexpr (KIND == EPI_QKV || KIND == EPI_RESID || KIND == EPI_GLU || KIND == EPI_STORE) {
         if (fn) {
             YK_CHECK_CUDA(cudaLaunchKernelEx(&cfg, gemm_tc_kernel<KIND, true>, *tmW, *tmX, a));
             return YK_OK;
@@ -1212,7 +1212,7 @@ yk_status gemm_run(yk_model* m, const void* W, const CUtensorMap* tmW, const voi
     }
     cfg.attrs = at;
     cfg.numAttrs = na;
-    // fused norm: the residual kind writes x / sums of squares, QKV and gate/up consume them
+    // fused norm: the residual kind writes x / sums of squares, QKV (or its plain store) and gate/up consume them
     const bool fn = ep.kind == EPI_RESID ? ep.nx_out != nullptr : (ep.in_ss != nullptr);
     if (fn && ep.kind == EPI_RESID) YK_ARG(ep.nx_g && ep.nx_ss && ep.ss_ld >= m_tok, "fused norm: outputs");
     if (fn && ep.kind != EPI_RESID) YK_ARG(m_tok <= TC_QKV_STAGE_TOK && ep.ss_ld >= m_tok, "fused norm: input");
@@ -1221,7 +1221,7 @@ yk_status gemm_run(yk_model* m, const void* W, const CUtensorMap* tmW, const voi
         case EPI_RESID: YK_TRY(launch_tc<EPI_RESID>(cfg, tmW, tmX, a, fn)); break;
         case EPI_GLU: YK_TRY(launch_tc<EPI_GLU>(cfg, tmW, tmX, a, fn)); break;
         case EPI_LOGITS: YK_TRY(launch_tc<EPI_LOGITS>(cfg, tmW, tmX, a, false)); break;
-        default: YK_TRY(launch_tc<EPI_STORE>(cfg, tmW, tmX, a, false)); break;
+        default: YK_TRY(launch_tc<EPI_STORE>(cfg, tmW, tmX, a, fn)); break;
     }
     e->launches++;
     return YK_OK;

@@ -145,6 +145,8 @@ struct LayerWeights {
     void* wdown = nullptr;  // [d x F]
     float* n1 = nullptr;    // [d]
     float* n2 = nullptr;    // [d]
+    float* qn = nullptr;    // [dh] per-head norms (yk_model_enable_qk_norm), else null
+    float* kn = nullptr;    // [dh]
     CUtensorMap tm_qkv, tm_o, tm_gu, tm_down;
 };
 
@@ -207,6 +209,12 @@ struct yk_model {
     int attn_counter_cap = 0;
     unsigned long long* attn_stamps = nullptr;  // test hook: per-CTA phase stamps, else null
     int attn_stamps_cap = 0, attn_last_items = 0;
+    bool qk_norm = false;
+    // raw projections of a step whose queries and keys are normed per head, or whose pool has 8-bit
+    // cells (allocated at the first one), and the workspace of attention over such a pool
+    float* qkv_raw = nullptr;   // [max_tokens x (H + 2 Hkv) dh]
+    uint8_t* attn8_ws = nullptr;
+    size_t attn8_ws_bytes = 0;
     // TMA maps of activation buffers, keyed by (buffer, token-box rows)
     std::map<std::pair<const void*, int>, CUtensorMap> xmaps;
     std::vector<void*> allocations;
@@ -217,6 +225,8 @@ struct yk_kv_pool {
     yk_model_config cfg{};
     int32_t num_blocks = 0;
     size_t esize = 4;
+    int32_t cells = YK_KV_F32; // YK_KV_*
+    uint8_t* scales = nullptr; // YK_KV_E4M3: [block][layer][2][Hkv]
     void* data = nullptr;      // [block][layer][2][Hkv][16][dh]
     size_t block_elems = 0;    // elements per block (all layers)
     size_t layer_elems = 0;    // elements per layer within a block
@@ -371,6 +381,12 @@ const uint32_t* sampler_device_drafts(const yk_sampler* s, int B, int* k);
 // add: a pending residual [rows of h x d] added to h first (fp32, or bf16 when add_bf16)
 yk_status launch_rmsnorm(yk_model* m, const float* g, int rows, const int32_t* row_idx, const void* add = nullptr,
                          int add_bf16 = 0);
+// The pool's memory as the operators see it.
+inline yk_kv_pages pool_pages(const yk_kv_pool* p) {
+    return {p->data, p->scales, p->cells, p->num_blocks, p->n_pool_layers, p->cfg.n_kv_heads, p->cfg.head_dim};
+}
+// N(0, std) values into every cell of an e4m3 pool.
+yk_status launch_fill_e4m3(yk_kv_pool* p, uint64_t seed, float std);
 // In-place sum over the tensor-parallel group of `count` fp32 (or bf16) values on the engine stream.
 yk_status tp_allreduce(yk_engine* e, void* buf, size_t count, bool bf16);
 // The group's own bf16 all-reduce: `count` values this rank wrote into tp_ar_slot

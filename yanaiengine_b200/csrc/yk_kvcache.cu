@@ -312,6 +312,43 @@ static cudaError_t launch_append_dh(cudaStream_t st, bool pdl, int sms, const Ap
     return launch_on(st, pdl, kv_append_kernel<SRC, DST, E4M3, DH, 1>, row_blocks + blocks, 128, smem, p, row_blocks, tile);
 }
 
+// N(0, std) into every cell of an e4m3 pool: one warp per (block, layer, K|V, head).
+__global__ void __launch_bounds__(128) fill_e4m3_kernel(uint8_t* cells, uint8_t* scales, long long heads, int dh, uint64_t seed, float std) {
+    const long long i = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (i >= heads) return;
+    const auto four = [&](int q) {  // values 4 q .. 4 q + 3 of this head (Box-Muller)
+        const uint4 r = philox4x32_10(make_uint4((uint32_t)i, (uint32_t)(i >> 32), (uint32_t)q, 0x4B38u),
+                                      make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
+        float4 v;
+        const float a = sqrtf(-2.f * logf(u24(r.x) + 2.98e-8f)) * std, b = sqrtf(-2.f * logf(u24(r.z) + 2.98e-8f)) * std;
+        sincospif(2.f * u24(r.y), &v.y, &v.x);
+        sincospif(2.f * u24(r.w), &v.w, &v.z);
+        return make_float4(v.x * a, v.y * a, v.z * b, v.w * b);
+    };
+    float amax = 0.f;
+    for (int q = lane; q < 4 * dh; q += 32) {
+        const float4 v = four(q);
+        amax = fmaxf(fmaxf(fmaxf(amax, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int e = kv8_cover(amax);
+    const float f = exp2_int(-e);
+    for (int q = lane; q < 4 * dh; q += 32) {
+        const float4 v = four(q);
+        reinterpret_cast<uint32_t*>(cells + i * 16 * dh)[q] = e4m3x2_from(v.x * f, v.y * f) | e4m3x2_from(v.z * f, v.w * f) << 16;
+    }
+    if (lane == 0) scales[i] = (uint8_t)(e + KV8_BIAS);
+}
+yk_status launch_fill_e4m3(yk_kv_pool* p, uint64_t seed, float std) {
+    const long long heads = (long long)p->num_blocks * p->n_pool_layers * 2 * p->cfg.n_kv_heads;
+    fill_e4m3_kernel<<<(unsigned)((heads + 3) / 4), 128, 0, p->e->stream>>>((uint8_t*)p->data, p->scales, heads, p->cfg.head_dim, seed, std);
+    p->e->launches++;
+    YK_CHECK_CUDA(cudaGetLastError());
+    return YK_OK;
+}
+
 template <typename SRC, typename DST, bool E4M3>
 static cudaError_t launch_append(cudaStream_t st, bool pdl, int sms, int dh, const AppendParams& p) {
     switch (dh) {

@@ -657,7 +657,8 @@ yk_status load_one(yk_model* m, Stager& sg, int32_t t, int32_t layer, const Sour
     return upload<float>(m, sg, L, w, s);
 }
 
-bool is_norm(int32_t t) { return t == YK_T_NORM1 || t == YK_T_NORM2 || t == YK_T_FINAL_NORM; }
+bool is_head_norm(int32_t t) { return t == YK_T_QNORM || t == YK_T_KNORM; }
+bool is_norm(int32_t t) { return t == YK_T_NORM1 || t == YK_T_NORM2 || t == YK_T_FINAL_NORM || is_head_norm(t); }
 
 }  // namespace
 
@@ -683,7 +684,8 @@ static bool hf_tensor(const std::string& name, int n_layers, int32_t* t, int32_t
         {"self_attn.v_proj.weight", YK_T_WV},  {"self_attn.o_proj.weight", YK_T_WO},
         {"mlp.gate_proj.weight", YK_T_WGATE},  {"mlp.up_proj.weight", YK_T_WUP},
         {"mlp.down_proj.weight", YK_T_WDOWN},  {"input_layernorm.weight", YK_T_NORM1},
-        {"post_attention_layernorm.weight", YK_T_NORM2}};
+        {"post_attention_layernorm.weight", YK_T_NORM2}, {"self_attn.q_norm.weight", YK_T_QNORM},
+        {"self_attn.k_norm.weight", YK_T_KNORM}};
     for (const auto& g : kGlobal)
         if (name == g.first) {
             *t = g.second;
@@ -725,19 +727,19 @@ extern "C" yk_status yk_model_load_safetensors(yk_model* m, yk_safetensors* cons
     const auto& c = m->cfg;
     const int L = c.n_layers;
     // every (tensor, layer) slot: which file holds it
-    std::vector<std::pair<const yk_safetensors*, const yk_safetensors::Entry*>> slot((size_t)(3 + 9 * L),
+    std::vector<std::pair<const yk_safetensors*, const yk_safetensors::Entry*>> slot((size_t)(3 + 11 * L),
                                                                                      {nullptr, nullptr});
     auto slot_of = [&](int32_t t, int32_t l) -> size_t {
         if (t == YK_T_EMBED) return 0;
         if (t == YK_T_FINAL_NORM) return 1;
         if (t == YK_T_LM_HEAD) return 2;
-        return 3 + (size_t)l * 9 + (size_t)(t - YK_T_WQ);
+        return 3 + (size_t)l * 11 + (size_t)(is_head_norm(t) ? 9 + t - YK_T_QNORM : t - YK_T_WQ);
     };
     for (int f = 0; f < n_files; ++f) {
         YK_ARG(files[f], "null file handle");
         for (const auto& e : files[f]->entries) {
             int32_t t, l;
-            if (!hf_tensor(e.name, L, &t, &l)) {
+            if (!hf_tensor(e.name, L, &t, &l) || (is_head_norm(t) && !m->qk_norm)) {
                 // buffers that are not weights of this module's layers are skipped;
                 // an unknown tensor of a decoder layer is a layer this module lacks
                 if (e.name.compare(0, 13, "model.layers.") == 0 && e.name.find("rotary_emb") == std::string::npos) {
@@ -759,8 +761,8 @@ extern "C" yk_status yk_model_load_safetensors(yk_model* m, yk_safetensors* cons
     Stager sg(m->e);
     YK_TRY(sg.init());
     int32_t loaded = 0;
-    for (int32_t t = 0; t <= YK_T_LM_HEAD; ++t) {
-        const bool per_layer = t >= YK_T_WQ && t <= YK_T_NORM2;
+    for (int32_t t = 0; t <= (m->qk_norm ? YK_T_KNORM : YK_T_LM_HEAD); ++t) {
+        const bool per_layer = (t >= YK_T_WQ && t <= YK_T_NORM2) || is_head_norm(t);
         for (int32_t l = 0; l < (per_layer ? L : 1); ++l) {
             const auto& s = slot[slot_of(t, l)];
             if (!s.first) {
@@ -785,6 +787,15 @@ extern "C" yk_status yk_model_load_safetensors(yk_model* m, yk_safetensors* cons
             }
             if ((flags & YK_LOAD_ROPE_HALF) && (t == YK_T_WQ || t == YK_T_WK)) src.rope_heads_hd = c.head_dim;
             if (is_norm(t)) src.add = norm_offset;
+            // a per-head gain follows its head's rows out of rotate-half order
+            std::vector<uint8_t> turned;
+            if ((flags & YK_LOAD_ROPE_HALF) && is_head_norm(t) && src.rows == 1 && src.cols == (size_t)c.head_dim) {
+                const size_t es = e.dtype == YK_DTYPE_F32 ? 4 : 2, half = src.cols / 2;
+                turned.resize(src.cols * es);
+                for (size_t k = 0; k < src.cols; ++k)
+                    std::memcpy(turned.data() + k * es, src.p + ((k & 1) * half + k / 2) * es, es);
+                src.p = turned.data();
+            }
             const yk_status st = load_one(m, sg, t, l, src);
             if (st != YK_OK) {
                 yk_set_error("loading '" + e.name + "': " + [] {
