@@ -10,17 +10,19 @@
 //   queries    the next span's queries into e4m3 pairs
 //   MMA        S^T[128 keys x 2R] = K Q^T (kind::f8f6f4), O^T[dims x R] += V^T P^T
 //              (kind::f16), accumulators in TMEM, S^T and O^T double-buffered
-//   softmax    8 warps, one key and half of the rows a thread: scores from TMEM,
-//              weights to shared memory
+//   softmax    two groups of 4 warps, half of the rows each, one key a thread: scores
+//              from TMEM, weights to shared memory
 //   V          4 warps: e4m3 V to f16, still [key][dim] (the MN-major operand of
 //              O^T); at a span's end they read O^T and write the result
 // K goes to the tensor core as it lies in the cache: no conversion at all.  The
-// queries, as bf16, are 8 bits wide: two e4m3 terms, the second scaled by 16,
-// hold them exactly (to 2^-21 of a row's largest value at least), as separate
-// columns of one product.  V converts once for all rows of the tile (R up to 64).
+// queries, as bf16, are 8 bits wide: two terms hold them exactly (to 2^-20.8 of a
+// row's largest value at least).  For few rows both are e4m3, the second scaled by
+// 16, as separate columns of one product; from 24 rows on the second is e5m2 (the
+// remainder is at most 8 units of the last bit, 3 bits wide) and its product adds
+// to the first's: half the scores to read back (prompt 835 -> 813 us).  V converts once for all rows of the tile (R up to 64).
 //
-// Weights as in the other kernel: p = 2^(x + e_V - m), f16.  The reference m is
-// common to the CTA and kept lazily: it is set 2^3 below a row's first weights
+// Weights as in the other kernel: p = 2^(x + e_V - m), f16.  The reference m of a
+// row is kept by its group, lazily: it is set 2^3 below a row's first weights
 // and moves when one would pass 2^15 (each move waits for the products before it
 // and rescales O^T in TMEM).  What lies 2^-28 below a row's largest weight is
 // lost: f16 ends at 2^-25, rounded.
@@ -56,7 +58,8 @@ struct TcaCfg {
     static constexpr int TILES = ROOM / KT;                    // K and V tiles that fit
     static constexpr int NV = TILES / 2 < 6 ? TILES / 2 : 6, NK = TILES - NV < 6 ? TILES - NV : 6;
     static constexpr int SMEM = 1024 + (NK + NV) * KT + NV16 * V16 + 2 * PB + 2 * QB + SMALL;
-    static constexpr int S_COLS = 2 * R, O_COLS = HALVES * RP;
+    static constexpr bool JOINED = R >= 24;                    // the queries' second terms: a product of their own
+    static constexpr int S_COLS = JOINED ? (R + 15) / 16 * 16 : 2 * R, O_COLS = HALVES * RP;
     static constexpr int COLS = 2 * S_COLS + 2 * O_COLS;
     static constexpr int TMEM = COLS <= 32 ? 32 : COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
     static_assert(NK >= 2 && NV >= 1 && COLS <= 512, "tile shapes");
@@ -121,17 +124,17 @@ __device__ __forceinline__ void mma_tc(uint32_t d, uint32_t a_lo, uint32_t a_hi,
             "r"(idesc), "r"(accumulate)
             : "memory");
 }
-// Barriers of the 8 softmax warps (true if any thread says so) and of the 4 V warps.
-__device__ __forceinline__ bool softmax_or(bool v) {
+// Barriers of the 4 warps of a softmax group (true if any thread says so) and of the 4 V warps.
+__device__ __forceinline__ bool softmax_or(int group, bool v) {
     uint32_t r;
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
         : "=r"(r)
-        : "r"((uint32_t)v)
+        : "r"(3 + group), "r"((uint32_t)v)
         : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_bar() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void softmax_bar(int group) { asm volatile("bar.sync %0, 128;" ::"r"(3 + group) : "memory"); }
 __device__ __forceinline__ void v_bar() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 __device__ __forceinline__ float warp_fmax(float v) {  // (NaN is passed over)
     float r;
@@ -164,6 +167,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+__device__ __forceinline__ uint32_t e5m2x2_from(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 __device__ __forceinline__ void sts64(uint32_t a, uint32_t x, uint32_t y) {
     asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(a), "r"(x), "r"(y) : "memory");
@@ -340,8 +348,9 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
         const int nseg = min(A8_SEGS, work.nspans - seg0);
         if (warp < 8) {
             // ---------------- softmax: key 32 * quad + lane of each tile, rows r0 .. r0 + RH - 1 ----------------
-            constexpr int RH = C::RH, BATCH = RH > 16 ? 8 : RH;  // rows read from TMEM at a time
-            const int quad = warp & 3, r0 = (warp >> 2) * RH, key = 32 * quad + lane;
+            constexpr int RH = C::RH, BATCH = RH % 16 == 0 ? 16 : RH > 16 ? 8 : RH;  // rows read from TMEM at a time
+            const int quad = warp & 3, group = warp >> 2, r0 = group * RH, key = 32 * quad + lane;
+            const int own = key < RH ? r0 + key : -1;  // a row whose reference this thread keeps
             const uint32_t lanes = (uint32_t)(32 * quad) << 16;
             // this key's weights in P, [key][row], 16-byte chunks swizzled by the key
             const uint32_t p_sw = (uint32_t)(C::PROW == 128 ? key & 7 : C::PROW == 64 ? key >> 1 & 3 : key >> 2 & 1) << 4;
@@ -350,13 +359,13 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
             for (int si = 0; si < nseg; ++si) {
                 const Seg sg = segs[si];
                 const int rows = sg.rows, pos_last = sg.pos + div_rep(p, sg.rem + rows - 1);
-                if (threadIdx.x < R) {
-                    const int n = threadIdx.x;
+                if (own >= 0) {
+                    const int n = own;
                     s_neg[n] = 0.f;
                     s_set[n] = 0;
                     s_pos[n] = n < rows ? sg.pos + div_rep(p, sg.rem + n) : -0x40000000;  // (no key is seen)
                 }
-                softmax_bar();
+                softmax_bar(group);
                 const unsigned w = p.window > 0 ? (unsigned)p.window : 0x80000000u;
                 bool force = true;  // some row has not seen a key yet
                 float2 l[RH / 2];
@@ -373,15 +382,17 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     const int ek = here ? (info & 255) - 128 : 0, ev = here ? (info >> 8) - 128 : 0;
                     const float fk = exp2_int(ek), inv = exp2_int(-ev);
                     const float2 fk2 = make_float2(fk, fk), shift = make_float2((float)ev, (float)ev), inv2 = make_float2(inv, inv);
+                    // (soft-capped scores are capped, then shifted, below)
+                    const float2 now = p.cap <= 0.f ? make_float2(1.f, 1.f) : make_float2(0.f, 0.f), first = mul2(shift, now);
                     const bool plain = p.cap <= 0.f && all_seen(p, sg, pos_last, j0) && __all_sync(0xffffffffu, here);
                     const float* const rf = s_rf + qt.slot * R + r0;
                     const uint32_t at = col_s(st.slot) + lanes + (uint32_t)r0;
                     float2 d[RH / 2];  // score + e_V - reference, rows r0 + 2 n, + 1
 #pragma unroll
                     for (int b0 = 0; b0 < RH; b0 += BATCH) {
-                        uint32_t x[BATCH], y[BATCH];
+                        uint32_t x[BATCH], y[C::JOINED ? 1 : BATCH];
                         tmem_ld<BATCH>(at + (uint32_t)b0, x);
-                        tmem_ld<BATCH>(at + (uint32_t)(R + b0), y);
+                        if constexpr (!C::JOINED) tmem_ld<BATCH>(at + (uint32_t)(R + b0), y);
                         float4 f[BATCH / 4], m[BATCH / 4];  // (these come while the scores do)
 #pragma unroll
                         for (int n = 0; n < BATCH / 4; ++n) {
@@ -392,12 +403,12 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
 #pragma unroll
                         for (int n = 0; n < BATCH; n += 2) {
                             const float4 ff = f[n / 4], mm = m[n / 4];
-                            const float2 s = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f),
-                                                  make_float2(__uint_as_float(x[n]), __uint_as_float(x[n + 1])));
+                            float2 s = make_float2(__uint_as_float(x[n]), __uint_as_float(x[n + 1]));
+                            if constexpr (!C::JOINED)
+                                s = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f), s);
                             const float2 r = n & 2 ? make_float2(ff.z, ff.w) : make_float2(ff.x, ff.y);
-                            const float2 c = add2(shift, n & 2 ? make_float2(mm.z, mm.w) : make_float2(mm.x, mm.y));
-                            // (soft-capped scores are capped, then shifted, below)
-                            d[(b0 + n) / 2] = p.cap <= 0.f ? fma2(mul2(s, fk2), r, c) : mul2(mul2(s, fk2), r);
+                            const float2 c = fma2(n & 2 ? make_float2(mm.z, mm.w) : make_float2(mm.x, mm.y), now, first);
+                            d[(b0 + n) / 2] = fma2(mul2(s, fk2), r, c);
                         }
                     }
                     tc_fence_before();
@@ -428,7 +439,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
 #pragma unroll
                     for (int n = 0; n < RH / 2; ++n) top = fmaxf(top, fmaxf(d[n].x, d[n].y));
                     // move the references: at a row's first keys, and before a weight would pass 2^15
-                    if (softmax_or(force || top > 15.f)) {
+                    if (softmax_or(group, force || top > 15.f)) {
                         float most = 0.f;  // lane n: the warp's largest of row r0 + n
 #pragma unroll
                         for (int n = 0; n < RH; ++n) {
@@ -436,10 +447,10 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             most = lane == n ? x : most;
                         }
                         if (lane < RH) s_mx[quad * R + r0 + lane] = most;
-                        softmax_bar();
+                        softmax_bar(group);
                         bool unset = false;
-                        if (threadIdx.x < R) {
-                            const int n = threadIdx.x;
+                        if (own >= 0) {
+                            const int n = own;
                             const float x = fmaxf(fmaxf(s_mx[n], s_mx[R + n]), fmaxf(s_mx[2 * R + n], s_mx[3 * R + n]));
                             const float was = -s_neg[n];
                             const bool set = s_set[n] != 0;
@@ -450,7 +461,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             if (x > -INFINITY) s_set[n] = 1;
                             unset = n < rows && !set && x == -INFINITY;
                         }
-                        force = softmax_or(unset);
+                        force = softmax_or(group, unset);
 #pragma unroll
                         for (int n = 0; n < RH; n += 4) {
                             const float4 a = *reinterpret_cast<const float4*>(s_dm + r0 + n), f = *reinterpret_cast<const float4*>(s_f + r0 + n);
@@ -521,7 +532,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                     if ((lane & 7) == 0) s_l[(ot.slot * 4 + quad) * R + r0 + n + (lane >> 3)] = x;
                     __syncwarp();
                 }
-                if (threadIdx.x < R) s_mo[ot.slot * R + threadIdx.x] = -s_neg[threadIdx.x];
+                if (own >= 0) s_mo[ot.slot * R + own] = -s_neg[own];
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(l_full + 8 * ot.slot);
@@ -529,7 +540,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                 }
                 qt.next();
                 ot.next();
-                softmax_bar();  // (s_neg has been read)
+                softmax_bar(group);  // (s_neg has been read)
             }
         } else if (warp < 12) {
             // ---------------- V: e4m3 -> f16, and the results ----------------
@@ -782,8 +793,11 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                         const uint32_t d = col_s(st.slot);
 #pragma unroll
                         for (int ks = 0; ks < DH / 32; ++ks)
-                            mma_tc<true>(d, ka + (uint32_t)((ks >> 2) * (TCA_TILE * 8) + (ks & 3) * 2), hi_s,
-                                         qa + (uint32_t)((ks >> 2) * (2 * R * 8) + (ks & 3) * 2), hi_s, idesc_s, ks == 0 ? 0u : 1u);
+#pragma unroll
+                            for (int t = 0; t < (C::JOINED ? 2 : 1); ++t)  // (bit 10: B is e5m2)
+                                mma_tc<true>(d, ka + (uint32_t)((ks >> 2) * (TCA_TILE * 8) + (ks & 3) * 2), hi_s,
+                                             qa + (uint32_t)((ks >> 2) * (2 * R * 8) + t * (R * C::ROWB / 16) + (ks & 3) * 2), hi_s,
+                                             idesc_s | (uint32_t)t << 10, ks + t == 0 ? 0u : 1u);
                         tc_commit(s_full + 8 * st.slot);
                         tc_commit(k_empty + 8 * kt.slot);
                         if (i == n - 1) tc_commit(q_empty + 8 * qt.slot);
@@ -851,7 +865,8 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             const uint32_t h = e4m3x2_from(a, b);
                             const float2 back = f32x2(f16x2_lo(h));
                             hi[z] |= h << (16 * k);
-                            lo[z] |= e4m3x2_from((a - back.x) * 16.f, (b - back.y) * 16.f) << (16 * k);
+                            lo[z] |= (C::JOINED ? e5m2x2_from(a - back.x, b - back.y)
+                                                : e4m3x2_from((a - back.x) * 16.f, (b - back.y) * 16.f)) << (16 * k);
                         }
                     }
                     if (row < R && !dead) {
