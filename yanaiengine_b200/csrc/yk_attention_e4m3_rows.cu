@@ -50,20 +50,24 @@ __device__ __forceinline__ void settle(uint32_t (&x)[16]) {
     asm volatile("" : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]),
                       "+r"(x[9]), "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15]));
 }
+// Raw scores of a page with this word -> log2 domain (above zero: masked ones stay -inf).
+__device__ __forceinline__ float score_factor(int word, float rf) { return fmaxf(fminf(exp2_int((word & 255) - 128) * rf, A8_LARGEST), 1.18e-38f); }
 // Barriers of the two warps of 32 rows: barrier 3 + quad says that an even tile's references are decided, 7 + quad an odd one's.
 __device__ __forceinline__ void pair_wait(int group, int quad) { asm volatile("bar.sync %0, 64;" ::"r"(3 + 4 * group + quad) : "memory"); }
 __device__ __forceinline__ void pair_tell(int group, int quad) { asm volatile("bar.arrive %0, 64;" ::"r"(3 + 4 * group + quad) : "memory"); }
 
-// Scores that are capped or masked: into the log2 domain, capped, -inf where the row does not see the key.
+// Scores that are capped (then in the log2 domain) or masked: -inf where the row does not see the key.
 static __device__ __noinline__ void finish_scores(uint32_t s_at, const int* info, float rf, int pos, int j0, unsigned window, float cap, float cap_log2,
-                                           float inv_cap_log2) {
+                                                  float inv_cap_log2) {
 #pragma unroll 1
     for (int b = 0; b < TCA_PAGES; ++b) {
         uint32_t x[16];
-        tmem_ld<16>(s_at + 16 * b, x);
         const int w = info[b];
-        const float f = fminf(exp2_int(w >= 0 ? (w & 255) - 128 : 0) * rf, A8_LARGEST);
         const unsigned wk = w >= 0 ? window : 0u;
+        // (a page that all rows of the warp see whole stays as it is)
+        if (cap <= 0.f && __all_sync(0xffffffffu, (unsigned)(pos - j0 - 16 * b) < wk && (unsigned)(pos - j0 - 16 * b - 15) < wk)) continue;
+        tmem_ld<16>(s_at + 16 * b, x);
+        const float f = cap > 0.f ? score_factor(w >= 0 ? w : 128, rf) : 1.f;
         tmem_wait_ld();
         settle(x);
 #pragma unroll
@@ -194,91 +198,86 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                     tc_fence_after();
                     uint32_t x[2][16];
                     const float rf = s_rf[qt.slot * R + row];
-                    float f[TCA_PAGES];  // scores of a page -> log2 domain
-                    int ev[TCA_PAGES];
+                    bool raw = p.cap <= 0.f;  // the scores in TMEM are not in the log2 domain yet
                     {
                         const int4 a = *reinterpret_cast<const int4*>(info), b = *reinterpret_cast<const int4*>(info + 4);
-                        const int w[TCA_PAGES] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                        const bool plain = p.cap <= 0.f && all_seen(p, sg, pos_last, j0) && (a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) >= 0;
-                        if (!plain) finish_scores(s_at, info, rf, pos, j0, window, p.cap, p.cap_log2, p.inv_cap_log2);
-#pragma unroll
-                        for (int z = 0; z < TCA_PAGES; ++z) {
-                            ev[z] = w[z] >= 0 ? (w[z] >> 8) - 128 : 0;
-                            f[z] = plain ? fminf(exp2_int((w[z] & 255) - 128) * rf, A8_LARGEST) : 1.f;
-                        }
+                        if (!raw || !all_seen(p, sg, pos_last, j0) || (a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) < 0)
+                            finish_scores(s_at, info, rf, pos, j0, window, p.cap, p.cap_log2, p.inv_cap_log2);
                     }
-                    // the row's largest score + e_V
+                    // the row's largest score + e_V (two pages a turn; the next page's scores come while one's are used)
                     float top = -INFINITY;
                     tmem_ld<16>(s_at, x[0]);
+#pragma unroll 1
+                    for (int b = 0; b < TCA_PAGES; b += 2) {
+                        const int2 w = *reinterpret_cast<const int2*>(info + b);
 #pragma unroll
-                    for (int b = 0; b < TCA_PAGES; ++b) {
-                        uint32_t(&y)[16] = x[b & 1];
-                        tmem_wait_ld();
-                        settle(y);
-                        if (b + 1 < TCA_PAGES) tmem_ld<16>(s_at + 16 * (b + 1), x[(b + 1) & 1]);
-                        float most = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+                        for (int u = 0; u < 2; ++u) {
+                            uint32_t(&y)[16] = x[u];
+                            tmem_wait_ld();
+                            settle(y);
+                            tmem_ld<16>(s_at + (uint32_t)(16 * (b + u + 1) & 127), x[u ^ 1]);
+                            float most = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 #pragma unroll
-                        for (int z = 2; z < 16; z += 2) most = fmaxf(most, fmaxf(__uint_as_float(y[z]), __uint_as_float(y[z + 1])));
-                        top = fmaxf(top, fmaf(most, f[b], (float)ev[b]));
+                            for (int z = 2; z < 16; z += 2) most = fmaxf(most, fmaxf(__uint_as_float(y[z]), __uint_as_float(y[z + 1])));
+                            const int word = u ? w.y : w.x;
+                            top = fmaxf(top, fmaf(most, raw ? score_factor(word, rf) : 1.f, (float)(word >= 0 ? (word >> 8) - 128 : 0)));
+                        }
                     }
                     // the reference, after the tile before has decided: 2^3 below a row's first weights, and again before one
                     // would pass 2^15
                     if (t > 0) pair_wait(group ^ 1, quad);
                     float now = i == 0 ? A8_LOWEST : s_m[row];
-                    const bool over = top > now + 15.f;
-                    if (__any_sync(0xffffffffu, over)) {
-                        const float was = now;
-                        now = over ? top - 3.f : was;
-                        if (i > 0) {
-                            // O follows, once the products of the tile before are done
-                            const float g = ex2(was - now);
-                            wait(p_empty + 8 * (group ^ 1), ((t - 1) >> 1) & 1);
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < DH; c += 16) {
-                                tmem_ld<16>(o_at + (uint32_t)c, x[0]);
-                                tmem_wait_ld();
-                                settle(x[0]);
-#pragma unroll
-                                for (int z = 0; z < 16; ++z) x[0][z] = __float_as_uint(__uint_as_float(x[0][z]) * g);
-                                tmem_st<16>(o_at + (uint32_t)c, x[0]);
-                            }
-                            tmem_wait_st();
-                        }
-                    }
+                    const bool over = top > now + 15.f, moves = __any_sync(0xffffffffu, over) && i > 0;
+                    const float was = now;
+                    if (over) now = top - 3.f;
                     s_m[row] = now;
                     if (t + 1 < total) pair_tell(group, quad);
-                    tmem_ld<16>(s_at, x[0]);
                     l *= ex2(m - now);
                     m = now;
                     wait(p_empty + 8 * group, (use & 1) ^ 1);
                     tc_fence_after();
+#pragma unroll 1
+                    for (int b = 0; b < TCA_PAGES; b += 2) {
+                        const int2 w = *reinterpret_cast<const int2*>(info + b);
 #pragma unroll
-                    for (int b = 0; b < TCA_PAGES; ++b) {
-                        uint32_t(&y)[16] = x[b & 1];
-                        tmem_wait_ld();
-                        settle(y);
-                        if (b + 1 < TCA_PAGES) {
-                            tmem_ld<16>(s_at + 16 * (b + 1), x[(b + 1) & 1]);
-                        } else {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(s_empty + 8 * group);
-                        }
-                        const float2 ff = make_float2(f[b], f[b]);
-                        const float c = (float)ev[b] - now;
-                        const float2 cc = make_float2(c, c);
-                        float2 sum = make_float2(0.f, 0.f);
-                        uint32_t h[8];
+                        for (int u = 0; u < 2; ++u) {
+                            uint32_t(&y)[16] = x[u];
+                            tmem_wait_ld();
+                            settle(y);
+                            if (u == 0 || b + 2 < TCA_PAGES) tmem_ld<16>(s_at + (uint32_t)(16 * (b + u + 1)), x[u ^ 1]);
+                            const int word = u ? w.y : w.x, ev = word >= 0 ? (word >> 8) - 128 : 0;
+                            const float f = raw ? score_factor(word, rf) : 1.f, c = (float)ev - now;
+                            const float2 ff = make_float2(f, f), cc = make_float2(c, c);
+                            float2 sum = make_float2(0.f, 0.f);
+                            uint32_t h[8];
 #pragma unroll
-                        for (int z = 0; z < 16; z += 2) {
-                            const float2 d = fma2(make_float2(__uint_as_float(y[z]), __uint_as_float(y[z + 1])), ff, cc);
-                            const float2 e = make_float2(ex2(d.x), ex2(d.y));
-                            sum = add2(sum, e);
-                            h[z / 2] = f16x2_of(e.x, e.y);
+                            for (int z = 0; z < 16; z += 2) {
+                                const float2 d = fma2(make_float2(__uint_as_float(y[z]), __uint_as_float(y[z + 1])), ff, cc);
+                                const float2 e = make_float2(ex2(d.x), ex2(d.y));
+                                sum = add2(sum, e);
+                                h[z / 2] = f16x2_of(e.x, e.y);
+                            }
+                            l = fmaf(sum.x + sum.y, exp2_int(-ev), l);
+                            tmem_st<8>(p_at + (uint32_t)(8 * (b + u)), h);
                         }
-                        l = fmaf(sum.x + sum.y, exp2_int(-ev[b]), l);
-                        tmem_st<8>(p_at + (uint32_t)(8 * b), h);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s_empty + 8 * group);
+                    if (moves) {
+                        // O follows, once the products of the tile before are done (by now they mostly are)
+                        const float g = ex2(was - now);
+                        wait(p_empty + 8 * (group ^ 1), ((t - 1) >> 1) & 1);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < DH; c += 16) {
+                            tmem_ld<16>(o_at + (uint32_t)c, x[0]);
+                            tmem_wait_ld();
+                            settle(x[0]);
+#pragma unroll
+                            for (int z = 0; z < 16; ++z) x[0][z] = __float_as_uint(__uint_as_float(x[0][z]) * g);
+                            tmem_st<16>(o_at + (uint32_t)c, x[0]);
+                        }
                     }
                     tmem_wait_st();
                     tc_fence_before();
@@ -385,9 +384,12 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
             constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(TCA_TILE >> 3) << 17) | ((uint32_t)(R >> 4) << 24);
             constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | ((uint32_t)(R >> 4) << 24);
             constexpr uint32_t hi_s = desc_hi(8 * C::ROWB, DH == 64 ? 4 : 2), hi_v = desc_hi(1024, 2);
-            // O of the tile before: whether it is still to come, and begins or ends its span
-            bool pending = false, begins = false, ends = false;
+            // O of a tile comes after S of the second tile behind it: the scores' room is free a little before the
+            // weights are there.  What is still to come: tiles that begin or end their span, the older in bit 1
+            int pending = 0;
+            unsigned begin_bits = 0, end_bits = 0;
             const auto values = [&]() {
+                const bool begins = begin_bits >> (pending - 1) & 1, ends = end_bits >> (pending - 1) & 1;
                 if (begins) wait(o_empty, ot.phase ^ 1);
                 wait2(p_full + 8 * pt.slot, pt.phase, w_full + 8 * wt.slot, wt.phase);
                 tc_fence_after();
@@ -404,7 +406,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                 pt.next();
                 wt.next();
                 if (ends) ot.next();
-                pending = false;
+                --pending;
             };
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
@@ -430,14 +432,14 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                     if (lane == 0) mbar_arrive(s_full + 8 * st.slot);  // (passes on what this warp has seen: page words, factors)
                     kt.next();
                     st.next();
-                    if (pending) values();
-                    pending = true;
-                    begins = i == 0;
-                    ends = i == n - 1;
+                    if (pending == 2) values();
+                    ++pending;
+                    begin_bits = begin_bits << 1 | (i == 0 ? 1u : 0u);
+                    end_bits = end_bits << 1 | (i == n - 1 ? 1u : 0u);
                 }
                 qt.next();
             }
-            if (pending) values();
+            while (pending > 0) values();
         } else {
             // ---------------- queries: two terms of each row ----------------
 #pragma unroll 1
