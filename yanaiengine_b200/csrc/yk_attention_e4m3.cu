@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
     pdl_wait();
 
     A8Work work;
-    if (!a8_plan<A8_THREADS, 1>(p, R, rep, s_scan, work)) return;
+    if (!a8_plan<A8_THREADS, 1, 0>(p, R, rep, s_scan, work)) return;
 
     // per-thread places in a page: K rows sigma(r), sigma(r) + 8; V rows c, c + 4, c + 8, c + 12
     const int sigma = (r & 1) * 4 + (r >> 1);
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
     int in_slot = 0, in_phase = 1, out_slot = 0, out_phase = 0;  // of the ring: next to fill, next to read
     // the spans of this CTA's range, A8_SEGS of them at a time
     for (int seg0 = 0; seg0 < work.nspans; seg0 += A8_SEGS) {
-        a8_list<1>(p, R, rep, work, seg0, segs);
+        a8_list<1, 0>(p, R, rep, work, seg0, segs);
         __syncthreads();
         const int nseg = min(A8_SEGS, work.nspans - seg0);
         const int v0 = segs[0].v, v1 = segs[nseg - 1].v + segs[nseg - 1].n;

@@ -88,9 +88,11 @@ __device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& star
 }
 
 
-// A thread's sequences and this CTA's range of units, [lo, hi) of the spans laid end to end.
+// A thread's sequences and this CTA's range of units, [lo, hi) of the spans laid end to end.  A span has COST units
+// more than its pages fill, in front, for what it costs beside them: spans that come and go quickly count.
 struct A8Work {
     int b_lo, b_hi;
+    int start, n, ctx;    // of sequence b_lo
     unsigned units, at0;  // of the thread's sequences, and before them
     unsigned per, lo, hi;
     int ord0;             // spans before the thread's
@@ -99,7 +101,7 @@ struct A8Work {
 
 // Block-wide: the range from the lengths on the device (prefix sums over the
 // sequences, THREADS threads).  False: nothing for this CTA.
-template <int THREADS, int PU>
+template <int THREADS, int PU, int COST>
 __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, unsigned* s_scan, A8Work& w) {
     constexpr int WARPS = THREADS / 32;
     static_assert(2 * WARPS + 2 <= A8_SCAN, "scan words");
@@ -108,19 +110,25 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     w.b_lo = min(p.B, (int)threadIdx.x * per_thread);
     w.b_hi = min(p.B, w.b_lo + per_thread);
     w.units = 0;  // (the host sees to it that all pages together stay below 2^31)
+    w.start = w.n = w.ctx = 0;
     int spans = 0;
     for (int b = w.b_lo; b < w.b_hi; ++b) {
         int start;
         const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+        if (b == w.b_lo) {
+            w.start = start;
+            w.n = n;
+            w.ctx = ctx;
+        }
         if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
         for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
-            w.units += (unsigned)(span_of(p, n, ctx, qt, R, rep).units<PU>() * p.G);
+            w.units += (unsigned)((span_of(p, n, ctx, qt, R, rep).units<PU>() + COST) * p.G);
             spans += p.G;
         }
     }
     w.at0 = w.units;  // exclusive prefixes over the threads
     w.ord0 = spans;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned x = __shfl_up_sync(0xffffffffu, w.at0, o);
         const int y = __shfl_up_sync(0xffffffffu, w.ord0, o);
@@ -134,32 +142,32 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
         s_scan[WARPS + warp] = (unsigned)w.ord0;
     }
     __syncthreads();
-    unsigned total = 0;
-    w.at0 -= w.units;
-    w.ord0 -= spans;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) {
-        if (i < warp) {
-            w.at0 += s_scan[i];
-            w.ord0 += (int)s_scan[WARPS + i];
-        }
-        total += s_scan[i];
-    }
+    const unsigned wu = lane < WARPS ? s_scan[lane] : 0u, ws = lane < WARPS ? s_scan[WARPS + lane] : 0u;
+    const unsigned total = __reduce_add_sync(0xffffffffu, wu);
+    w.at0 += __reduce_add_sync(0xffffffffu, lane < warp ? wu : 0u) - w.units;
+    w.ord0 += (int)__reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u) - spans;
     w.per = max((unsigned)(A8_MIN_PAGES / PU), (total + gridDim.x - 1) / gridDim.x);
     w.lo = min(total, blockIdx.x * w.per);
     w.hi = min(total, w.lo + w.per);
     if (w.lo >= w.hi) return false;
-    // the first and the last span of the range: the threads that hold them say so
+    // the spans that the range begins and ends in: the threads that hold them say so
     if (w.at0 < w.hi && w.at0 + w.units > w.lo && (w.at0 <= w.lo || w.at0 + w.units >= w.hi)) {
         unsigned at = w.at0;
         int ord = w.ord0;
         for (int b = w.b_lo; b < w.b_hi; ++b) {
-            int start;
-            const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+            int start = w.start, n = w.n, ctx = w.ctx;
+            if (b > w.b_lo) {
+                n = new_tokens(p, b, start);
+                ctx = p.ctx[b];
+            }
             for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
-                const unsigned u = (unsigned)span_of(p, n, ctx, qt, R, rep).units<PU>(), end = at + u * p.G;
+                const unsigned u = (unsigned)span_of(p, n, ctx, qt, R, rep).units<PU>() + COST, end = at + u * p.G;
+                // (its last page's unit may lie behind the range already, or its first one still)
                 if (at <= w.lo && end > w.lo) s_scan[2 * WARPS] = (unsigned)ord + (w.lo - at) / u;
-                if (at < w.hi && end >= w.hi) s_scan[2 * WARPS + 1] = (unsigned)ord + (w.hi - at - 1) / u;
+                if (at < w.hi && end >= w.hi) {
+                    const unsigned i = (w.hi - at - 1) / u;
+                    s_scan[2 * WARPS + 1] = (unsigned)ord + i - (COST > 0 && at + i * u + COST >= w.hi ? 1u : 0u);
+                }
                 at = end;
                 ord += p.G;
             }
@@ -168,23 +176,26 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     __syncthreads();
     w.first = (int)s_scan[2 * WARPS];
     w.nspans = (int)s_scan[2 * WARPS + 1] - w.first + 1;
-    return true;
+    return w.nspans > 0;  // (a range may hold nothing but such a cost)
 }
 
 // Block-wide: spans seg0 .. seg0 + A8_SEGS - 1 of the range into segs (a barrier must follow).
-template <int PU>
-__device__ __noinline__ void a8_list(const Attn8Params& p, int R, int rep, const A8Work& w, int seg0, Seg* segs) {
+template <int PU, int COST>
+__device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, const A8Work& w, int seg0, Seg* segs) {
     if (w.at0 >= w.hi || w.at0 + w.units <= w.lo) return;
     unsigned at = w.at0;
     int ord = w.ord0 - w.first - seg0;  // place in segs
     for (int b = w.b_lo; b < w.b_hi; ++b) {
-        int start;
-        const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+        int start = w.start, n = w.n, ctx = w.ctx;
+        if (b > w.b_lo) {
+            n = new_tokens(p, b, start);
+            ctx = p.ctx[b];
+        }
         for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
             const Span s = span_of(p, n, ctx, qt, R, rep);
-            const unsigned u = (unsigned)s.units<PU>();
+            const unsigned u = (unsigned)s.units<PU>() + COST;
             for (int g = max(0, -ord); g < min(p.G, A8_SEGS - ord); ++g) {
-                const unsigned from = at + g * u, to = from + u;
+                const unsigned from = at + g * u + COST, to = from + u - COST;
                 if (to <= w.lo || from >= w.hi) continue;
                 Seg x;
                 x.b = b;

@@ -140,10 +140,9 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
     for (int i = threadIdx.x; i < R * (DH / 32); i += TCR_THREADS) s_nan[i] = 0;
     pdl_wait();
     A8Work work;
-    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES>(p, R, rep, s_scan, work);  // (block-uniform)
+    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
     if (!busy) return;
     if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
-    a8_list<TCA_PAGES>(p, R, rep, work, 0, segs);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -170,19 +169,16 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
     int tile = 0;  // of this CTA
 
     for (int seg0 = 0; seg0 < work.nspans; seg0 += A8_SEGS) {
-        if (seg0 > 0) {
-            __syncwarp();
-            __syncthreads();
-            a8_list<TCA_PAGES>(p, R, rep, work, seg0, segs);
-            __syncthreads();
-        }
+        __syncwarp();
+        __syncthreads();
+        a8_list<TCA_PAGES, TCA_COST>(p, R, rep, work, seg0, segs);
+        __syncthreads();
         const int nseg = min(A8_SEGS, work.nspans - seg0);
         if (warp < 8) {
             // ---------------- softmax: row 32 * quad + lane; group 0 takes the even tiles, group 1 the odd ones ----------------
             const int quad = warp & 3, group = warp >> 2, row = 32 * quad + lane;
             const uint32_t lanes = (uint32_t)(32 * quad) << 16;
             const uint32_t s_at = col_s(group) + lanes, p_at = col_p(group) + lanes, o_at = col_o + lanes;
-            const int total = (int)(work.hi - work.lo);
             const unsigned window = p.window > 0 ? (unsigned)p.window : 0x80000000u;
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
@@ -231,7 +227,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                     const float was = now;
                     if (over) now = top - 3.f;
                     s_m[row] = now;
-                    if (t + 1 < total) pair_tell(group, quad);
+                    if (i + 1 < n || si + 1 < nseg || seg0 + A8_SEGS < work.nspans) pair_tell(group, quad);  // (not after the last tile)
                     l *= ex2(m - now);
                     m = now;
                     wait(p_empty + 8 * group, (use & 1) ^ 1);

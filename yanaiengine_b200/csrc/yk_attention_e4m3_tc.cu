@@ -147,10 +147,9 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
     for (int i = threadIdx.x; i < R * (DH / 32); i += TCA_THREADS) s_nan[i] = 0;
     pdl_wait();
     A8Work work;
-    const bool busy = a8_plan<TCA_THREADS, TCA_PAGES>(p, R, rep, s_scan, work);  // (block-uniform)
+    const bool busy = a8_plan<TCA_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
     if (!busy) return;
     if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
-    a8_list<TCA_PAGES>(p, R, rep, work, 0, segs);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -177,12 +176,10 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
     int tile = 0;           // of this CTA (page words)
 
     for (int seg0 = 0; seg0 < work.nspans; seg0 += A8_SEGS) {
-        if (seg0 > 0) {
-            __syncwarp();
-            __syncthreads();
-            a8_list<TCA_PAGES>(p, R, rep, work, seg0, segs);
-            __syncthreads();
-        }
+        __syncwarp();
+        __syncthreads();
+        a8_list<TCA_PAGES, TCA_COST>(p, R, rep, work, seg0, segs);
+        __syncthreads();
         const int nseg = min(A8_SEGS, work.nspans - seg0);
         if (warp < 8) {
             // ---------------- softmax: key 32 * quad + lane of each tile, rows r0 .. r0 + RH - 1 ----------------

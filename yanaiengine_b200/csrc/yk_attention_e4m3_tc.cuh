@@ -7,6 +7,7 @@ namespace yk {
 
 constexpr int TCA_TILE = 128;  // keys
 constexpr int TCA_PAGES = TCA_TILE / YK_BLOCK_SIZE;
+constexpr int TCA_COST = 2;    // a span's own cost, in tiles (verify: 6000 cycles and 2700 for a tile; head_dim 64: 2700 and 1600)
 constexpr int TCA_INFO = 16;   // tiles whose page words are kept
 
 // ---------------------------------------------------------------------------
