@@ -67,15 +67,21 @@ struct Span {
     template <int PU>  // in units of PU pages
     __device__ __forceinline__ int units() const { return max(1, (pend - page + PU - 1) / PU); }
 };
+// Query tiles of n new tokens (n may be -1).  R is a constant wherever this is called from a kernel's one shape.
+__device__ __forceinline__ int tiles_of(int n, int R, int rep) { return n <= 0 ? 0 : (int)(((unsigned)n * (unsigned)rep + (unsigned)R - 1u) / (unsigned)R); }
 __device__ __forceinline__ Span span_of(const Attn8Params& p, int n, int ctx, int qt, int R, int rep) {
-    const long long lo = (long long)qt * R;
+    // (32 bits hold all of this: the host sees to T * n_heads < 2^31 and max_blocks * 16 <= 2^29)
+    const unsigned lo = (unsigned)qt * (unsigned)R;
     Span s;
-    s.rows = (int)min((long long)n * rep - lo, (long long)R);
-    s.tok = qt == 0 ? 0 : (int)((unsigned)lo / (unsigned)rep);
-    s.rem = (int)lo - s.tok * rep;
+    s.rows = (int)min((unsigned)n * (unsigned)rep - lo, (unsigned)R);
+    s.tok = s.rem = 0;
+    if (qt > 0) {
+        s.tok = (int)(lo / (unsigned)rep);
+        s.rem = (int)lo - s.tok * rep;
+    }
     const int first = ctx - n + s.tok;
     const int last = first + div_rep(p, s.rem + s.rows - 1);
-    s.pend = (int)((min(max((long long)last + 1, 0LL), (long long)p.max_blocks * 16) + 15) >> 4);
+    s.pend = (min(max(last, -1), p.max_blocks * 16 - 1) + 16) >> 4;
     s.page = p.window > 0 ? min(max(0, first - p.window + 1) >> 4, s.pend) : 0;
     return s;
 }
@@ -121,7 +127,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
             w.ctx = ctx;
         }
         if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
-        for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+        for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
             w.units += (unsigned)((span_of(p, n, ctx, qt, R, rep).units<PU>() + COST) * p.G);
             spans += p.G;
         }
@@ -160,7 +166,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
                 n = new_tokens(p, b, start);
                 ctx = p.ctx[b];
             }
-            for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+            for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
                 const unsigned u = (unsigned)span_of(p, n, ctx, qt, R, rep).units<PU>() + COST, end = at + u * p.G;
                 // (its last page's unit may lie behind the range already, or its first one still)
                 if (at <= w.lo && end > w.lo) s_scan[2 * WARPS] = (unsigned)ord + (w.lo - at) / u;
@@ -191,7 +197,7 @@ __device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, co
             n = new_tokens(p, b, start);
             ctx = p.ctx[b];
         }
-        for (int qt = 0; (long long)qt * R < (long long)n * rep; ++qt) {
+        for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
             const Span s = span_of(p, n, ctx, qt, R, rep);
             const unsigned u = (unsigned)s.units<PU>() + COST;
             for (int g = max(0, -ord); g < min(p.G, A8_SEGS - ord); ++g) {
@@ -208,8 +214,9 @@ __device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, co
                 x.pend = s.pend;
                 x.v = (int)(max(from, w.lo) - w.lo);
                 x.n = (int)(min(to, w.hi) - max(from, w.lo));
-                x.c0 = (int)blockIdx.x - (from >= w.lo ? 0 : (int)((w.lo - from + w.per - 1) / w.per));
-                x.c1 = (int)blockIdx.x + (to <= w.hi ? 0 : (int)((to - 1 - w.lo) / w.per));
+                x.c0 = x.c1 = (int)blockIdx.x;
+                if (from < w.lo) x.c0 -= (int)((w.lo - from + w.per - 1) / w.per);
+                if (to > w.hi) x.c1 += (int)((to - 1 - w.lo) / w.per);
                 segs[ord + g] = x;
             }
             at += u * p.G;

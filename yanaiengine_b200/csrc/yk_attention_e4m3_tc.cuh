@@ -280,13 +280,9 @@ __device__ __forceinline__ void copy_tiles(const Attn8Params& p, const CUtensorM
             const bool mine = lane >> 3 == (i & 3);  // this lane's page belongs to the tile
             const int pages = __popc(__ballot_sync(0xffffffffu, mine && id >= 0));
             const uint32_t bar = full + 8 * t.slot;
-            if (mine)
-                info[(tile & (TCA_INFO - 1)) * TCA_PAGES + (lane & 7)] =
-                    id < 0 ? -1 : (kv8_exponent(kb) + 128) | (kv8_exponent(vb) + 128) << 8;
             wait(empty + 8 * t.slot, t.phase ^ 1);
             __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(bar, dead ? 0u : (uint32_t)(pages * 16 * DH));
-            __syncwarp();
+            // (the copies first: the scale bytes may still be on their way, and the barrier's one arrival comes after both)
             if (mine && id >= 0 && !dead) {
                 const uint32_t dst = smem_u32(ring + t.slot * TCA_TILE * DH) + (uint32_t)((lane & 7) * 16 * (V ? DH : ROWB));
                 if constexpr (V) {
@@ -301,6 +297,11 @@ __device__ __forceinline__ void copy_tiles(const Attn8Params& p, const CUtensorM
                             : "memory");
                 }
             }
+            if (mine)
+                info[(tile & (TCA_INFO - 1)) * TCA_PAGES + (lane & 7)] =
+                    id < 0 ? -1 : (kv8_exponent(kb) + 128) | (kv8_exponent(vb) + 128) << 8;
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(bar, dead ? 0u : (uint32_t)(pages * 16 * DH));
             t.next();
         }
     }
