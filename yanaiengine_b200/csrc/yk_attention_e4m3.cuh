@@ -98,7 +98,8 @@ __device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& star
 // more than its pages fill, in front, for what it costs beside them: spans that come and go quickly count.
 struct A8Work {
     int b_lo, b_hi;
-    int start, n, ctx;    // of sequence b_lo
+    int start, n, ctx;    // of sequence b_lo ...
+    int q_lo, q_hi;       // ... and the query tiles of it that are the thread's (of further sequences: all)
     unsigned units, at0;  // of the thread's sequences, and before them
     unsigned per, lo, hi;
     int ord0;             // spans before the thread's
@@ -112,11 +113,13 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     constexpr int WARPS = THREADS / 32;
     static_assert(2 * WARPS + 2 <= A8_SCAN, "scan words");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // many query tiles to a sequence: 2^share threads to each; more sequences than threads: several to a thread
     const int per_thread = (p.B + THREADS - 1) / THREADS;
-    w.b_lo = min(p.B, (int)threadIdx.x * per_thread);
+    const int share = p.B >= THREADS || p.T * rep <= 2 * R * p.B ? 0 : 31 - __clz(THREADS / p.B);
+    w.b_lo = min(p.B, (int)(threadIdx.x >> share) * per_thread);
     w.b_hi = min(p.B, w.b_lo + per_thread);
     w.units = 0;  // (the host sees to it that all pages together stay below 2^31)
-    w.start = w.n = w.ctx = 0;
+    w.start = w.n = w.ctx = w.q_lo = w.q_hi = 0;
     int spans = 0;
     for (int b = w.b_lo; b < w.b_hi; ++b) {
         int start;
@@ -125,9 +128,13 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
             w.start = start;
             w.n = n;
             w.ctx = ctx;
+            const int tiles = tiles_of(n, R, rep), each = (tiles + (1 << share) - 1) >> share;
+            w.q_lo = min(tiles, ((int)threadIdx.x & ((1 << share) - 1)) * each);
+            w.q_hi = min(tiles, w.q_lo + each);
         }
         if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
-        for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
+        const int q_hi = b == w.b_lo ? w.q_hi : tiles_of(n, R, rep);
+        for (int qt = b == w.b_lo ? w.q_lo : 0; qt < q_hi; ++qt) {
             w.units += (unsigned)((span_of(p, n, ctx, qt, R, rep).units<PU>() + COST) * p.G);
             spans += p.G;
         }
@@ -166,7 +173,8 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
                 n = new_tokens(p, b, start);
                 ctx = p.ctx[b];
             }
-            for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
+            const int q_hi = b == w.b_lo ? w.q_hi : tiles_of(n, R, rep);
+            for (int qt = b == w.b_lo ? w.q_lo : 0; qt < q_hi; ++qt) {
                 const unsigned u = (unsigned)span_of(p, n, ctx, qt, R, rep).units<PU>() + COST, end = at + u * p.G;
                 // (its last page's unit may lie behind the range already, or its first one still)
                 if (at <= w.lo && end > w.lo) s_scan[2 * WARPS] = (unsigned)ord + (w.lo - at) / u;
@@ -188,39 +196,48 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
 // Block-wide: spans seg0 .. seg0 + A8_SEGS - 1 of the range into segs (a barrier must follow).
 template <int PU, int COST>
 __device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, const A8Work& w, int seg0, Seg* segs) {
-    if (w.at0 >= w.hi || w.at0 + w.units <= w.lo) return;
-    unsigned at = w.at0;
-    int ord = w.ord0 - w.first - seg0;  // place in segs
-    for (int b = w.b_lo; b < w.b_hi; ++b) {
-        int start = w.start, n = w.n, ctx = w.ctx;
-        if (b > w.b_lo) {
-            n = new_tokens(p, b, start);
-            ctx = p.ctx[b];
-        }
-        for (int qt = 0; qt < tiles_of(n, R, rep); ++qt) {
-            const Span s = span_of(p, n, ctx, qt, R, rep);
-            const unsigned u = (unsigned)s.units<PU>() + COST;
-            for (int g = max(0, -ord); g < min(p.G, A8_SEGS - ord); ++g) {
-                const unsigned from = at + g * u + COST, to = from + u - COST;
-                if (to <= w.lo || from >= w.hi) continue;
-                Seg x;
-                x.b = b;
-                x.g = g;
-                x.tok = start + s.tok;
-                x.rem = s.rem;
-                x.rows = s.rows;
-                x.pos = ctx - n + s.tok;
-                x.page = s.page + PU * (int)(max(from, w.lo) - from);
-                x.pend = s.pend;
-                x.v = (int)(max(from, w.lo) - w.lo);
-                x.n = (int)(min(to, w.hi) - max(from, w.lo));
-                x.c0 = x.c1 = (int)blockIdx.x;
-                if (from < w.lo) x.c0 -= (int)((w.lo - from + w.per - 1) / w.per);
-                if (to > w.hi) x.c1 += (int)((to - 1 - w.lo) / w.per);
-                segs[ord + g] = x;
+    // A warp goes through those of its threads that hold some of them; its lanes take the KV heads.
+    const int lane = threadIdx.x & 31;
+    unsigned holders = __ballot_sync(0xffffffffu, w.at0 < w.hi && w.at0 + w.units > w.lo);
+    for (; holders; holders &= holders - 1) {
+        const int who = __ffs(holders) - 1;
+        unsigned at = __shfl_sync(0xffffffffu, w.at0, who);
+        int ord = __shfl_sync(0xffffffffu, w.ord0, who) - w.first - seg0;  // place in segs
+        const int b_lo = __shfl_sync(0xffffffffu, w.b_lo, who), b_hi = __shfl_sync(0xffffffffu, w.b_hi, who);
+        int start = __shfl_sync(0xffffffffu, w.start, who), n = __shfl_sync(0xffffffffu, w.n, who);
+        int ctx = __shfl_sync(0xffffffffu, w.ctx, who), q_lo = __shfl_sync(0xffffffffu, w.q_lo, who), q_hi = __shfl_sync(0xffffffffu, w.q_hi, who);
+        for (int b = b_lo; b < b_hi; ++b) {
+            if (b > b_lo) {
+                n = new_tokens(p, b, start);
+                ctx = p.ctx[b];
+                q_lo = 0;
+                q_hi = tiles_of(n, R, rep);
             }
-            at += u * p.G;
-            ord += p.G;
+            for (int qt = q_lo; qt < q_hi && ord < A8_SEGS && at < w.hi; ++qt) {
+                const Span s = span_of(p, n, ctx, qt, R, rep);
+                const unsigned u = (unsigned)s.units<PU>() + COST;
+                for (int g = max(0, -ord) + lane; g < min(p.G, A8_SEGS - ord); g += 32) {
+                    const unsigned from = at + g * u + COST, to = from + u - COST;
+                    if (to <= w.lo || from >= w.hi) continue;
+                    Seg x;
+                    x.b = b;
+                    x.g = g;
+                    x.tok = start + s.tok;
+                    x.rem = s.rem;
+                    x.rows = s.rows;
+                    x.pos = ctx - n + s.tok;
+                    x.page = s.page + PU * (int)(max(from, w.lo) - from);
+                    x.pend = s.pend;
+                    x.v = (int)(max(from, w.lo) - w.lo);
+                    x.n = (int)(min(to, w.hi) - max(from, w.lo));
+                    x.c0 = x.c1 = (int)blockIdx.x;
+                    if (from < w.lo) x.c0 -= (int)((w.lo - from + w.per - 1) / w.per);
+                    if (to > w.hi) x.c1 += (int)((to - 1 - w.lo) / w.per);
+                    segs[ord + g] = x;
+                }
+                at += u * p.G;
+                ord += p.G;
+            }
         }
     }
 }

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
     const uint32_t q_full = w_empty + 16, q_empty = q_full + 16, l_full = q_empty + 16, l_empty = l_full + 16;
     const uint32_t o_full = l_empty + 16, o_empty = o_full + 8;
     static_assert(2 * NK + 2 * NV + 22 <= 64, "barriers");
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 480) {  // (not of the warps that plan first)
         const auto init = [](uint32_t bar, int n, int count) {
             for (int i = 0; i < n; ++i) mbar_init(bar + 8 * i, (uint32_t)count);
         };
@@ -140,14 +140,17 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
     for (int i = threadIdx.x; i < R * (DH / 32); i += TCR_THREADS) s_nan[i] = 0;
     pdl_wait();
     A8Work work;
-    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
-    if (!busy) return;
     if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
+    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    pdl_trigger();  // (after the TMEM is taken: a kernel that starts early does not take it first)
     const uint32_t tmem = *s_tmem;
+    if (!busy) {
+        if (warp == 14) tmem_dealloc(tmem, C::TMEM);
+        return;
+    }
+    pdl_trigger();  // (after the TMEM is taken: a kernel that starts early does not take it first)
     const auto col_s = [&](int b) { return tmem + (uint32_t)(b * 128); };
     const auto col_p = [&](int b) { return tmem + (uint32_t)(256 + b * 64); };
     const uint32_t col_o = tmem + 384;
@@ -296,6 +299,11 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
             // ---------------- V: e4m3 -> f16, and the results ----------------
             const int tid = threadIdx.x - 256, quad = warp & 3;
             const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+            if (seg0 == 0) {
+                convert_queries<DH, R, true>(p, segs[0], rep, lane, quad, 5, s_q, s_rf, [] { return true; });
+                fence_proxy_async_smem();
+                first_queries_bar();
+            }
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
                 const Seg sg = segs[si];
@@ -440,9 +448,11 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
             // ---------------- queries: two terms of each row ----------------
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
-                convert_queries<DH, R, true>(p, segs[si], rep, lane, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
+                const bool first = seg0 + si == 0;
+                convert_queries<DH, R, true>(p, segs[si], rep, lane, first ? 4 : 0, first ? 5 : 1, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
                                              [&] { wait(q_empty + 8 * qt.slot, qt.phase ^ 1); return !dead; });
                 fence_proxy_async_smem();
+                if (first) first_queries_bar();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full + 8 * qt.slot);
                 qt.next();

@@ -161,6 +161,8 @@ struct Turn {
     }
 };
 
+// The V warps and the queries' warp: a CTA's first queries, which everything waits for, are converted by all five.
+__device__ __forceinline__ void first_queries_bar() { asm volatile("bar.sync 1, 160;" ::: "memory"); }
 __device__ __forceinline__ void v_bar() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 __device__ __forceinline__ float cap_score(const Attn8Params& p, float x) { return p.cap_log2 * tanh_cap(x * p.inv_cap_log2); }
 
@@ -307,12 +309,12 @@ __device__ __forceinline__ void copy_tiles(const Attn8Params& p, const CUtensorM
     }
 }
 
-// One warp: a span's queries as two terms that sum to them, [128-dim block][term][R rows][128 bytes] (head_dim 64:
+// A warp, part of `parts`: a span's queries as two terms that sum to them, [128-dim block][term][R rows][128 bytes] (head_dim 64:
 // 64 bytes), swizzled, and the rows' score factors.  JOINED: the second term is e5m2, else e4m3 times 16.
 // `free` waits until the room is, and says whether to write.
 template <int DH, int R, bool JOINED, typename Free>
-__device__ __forceinline__ void convert_queries(const Attn8Params& p, const Seg& sg, int rep, int lane, uint8_t* room, float* s_rf,
-                                                const Free& free) {
+__device__ __forceinline__ void convert_queries(const Attn8Params& p, const Seg& sg, int rep, int lane, int part, int parts, uint8_t* room,
+                                                float* s_rf, const Free& free) {
     constexpr int LPR = DH / 16, RPI = 32 / LPR;  // lanes a row, rows at a time
     const int c16 = lane % LPR;
     uint4 x[2], y[2];  // 16 values; the next rows' come while these convert
@@ -328,11 +330,11 @@ __device__ __forceinline__ void convert_queries(const Attn8Params& p, const Seg&
             v[1] = __ldcg(src + 1);
         }
     };
-    load(0, x);
+    load(part * RPI, x);
     const bool live = free();
 #pragma unroll 1
-    for (int r0 = 0; r0 < R; r0 += RPI) {
-        load(r0 + RPI, y);
+    for (int r0 = part * RPI; r0 < R; r0 += parts * RPI) {
+        load(r0 + parts * RPI, y);
         const int row = r0 + lane / LPR;
         float f[16];
         const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
