@@ -570,6 +570,157 @@ def test_append_pool_beyond_32_bit_offsets():
 
 
 # ---------------------------------------------------------------------------
+# The bf16 kernel for many rows (more than a tile of the other holds, by max_new): everything above again.
+# ---------------------------------------------------------------------------
+MANY = dict(max_new=1000)
+
+
+@pytest.mark.parametrize("H,G,dh", [(4, 4, 64), (8, 2, 64), (3, 1, 128), (8, 1, 128), (24, 8, 128), (64, 2, 64)])
+def test_many_rows_ragged(H, G, dh):
+    Attention(H * 100 + dh, H, G, dh, [(1, 1), (1, 16), (40, 57), (3, 3), (6, 160), (5, 33), (130, 700), (2, 1031)]).check(**MANY)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("window", [1, 2, 16, 37, 100, 5000])
+def test_many_rows_window(dh, window):
+    Attention(window, 8, 2, dh, [(6, 400), (1, 65), (40, 90), (5, 5), (70, 300)]).check(window=window, **MANY)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+def test_many_rows_cap_and_scale(dh):
+    Attention(5, 8, 4, dh, [(6, 400), (1, 65), (40, 40)], q_std=2.0).check(cap=30.0, scale=0.21, **MANY)
+    Attention(6, 8, 4, dh, [(6, 300), (1, 65), (40, 200)], q_std=2.0).check(cap=5.0, window=50, **MANY)
+
+
+def test_many_rows_padding_empty_and_below_zero():
+    Attention(9, 8, 2, 128, [(0, 40), (30, 40), (0, 0), (1, 20), (0, 16)], pad=5).check(**MANY)
+    a = Attention(11, 8, 2, 128, [(25, 40), (3, 40)])
+    a.ctx[0] = 2  # 25 new tokens, two positions: the first 23 have no key
+    a.check(**MANY)
+    assert (a.out[:23] == 0).all()
+
+
+@pytest.mark.parametrize("many", [0, 1])
+def test_more_spans_than_a_cta_lists_at_once(many):
+    rng = np.random.default_rng(1)
+    Attention(12, 8, 8, 64, [(1, int(c)) for c in rng.integers(1, 40, 700)]).check(max_new=1000 if many else 1)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+def test_many_rows_of_a_long_sequence_among_short_ones(dh):
+    """Its spans are cut between CTAs; the parts are joined the same way each time."""
+    a = Attention(13, 4, 2, dh, [(40, 9000)] + [(1, 3)] * 100 + [(33, 700)])
+    a.check(**MANY)
+    first = a.out.clone()
+    a.check(**MANY)
+    assert torch.equal(first, a.out)
+
+
+def test_many_rows_scales_far_apart():
+    a = Attention(14, 8, 2, 128, [(20, 200), (1, 90)], spread=0.0)
+    byte = torch.arange(a.scales.numel()).reshape(a.scales.shape) * 7 % 121 + 67
+    a.scales[:, :, 1] = byte.to(torch.uint8).to(dev())[:, :, 1]
+    a.check(**MANY)
+    a.scales[:, :, 1] = torch.tensor([0, 255], dtype=torch.uint8, device=dev())[torch.arange(2, device=dev())]
+    a.check(**MANY)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+def test_many_rows_nan_in_masked_cells(dh):
+    lens = [(6, 101), (1, 33), (20, 40), (17, 200)]
+    a = Attention(15, 8, 2, dh, lens)
+    want = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables, window=30)
+    for b, (n, c) in enumerate(lens):
+        for j in list(range(c, (c + 15) // 16 * 16)) + list(range(0, max(0, c - n - 30 + 1))):
+            a.pool[a.tables[b, j // 16], 1, :, :, j % 16] = 0x7F
+    a.call(window=30, **MANY)
+    torch.cuda.synchronize()
+    a.compare(*want)
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("which", [0, 1])
+def test_many_rows_nan_cell_reaches_those_who_see_it(dh, which):
+    a = Attention(16, 4, 2, dh, [(28, 60), (1, 20), (9, 300)])
+    want, weight, spread, floor = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
+    j = 60 - 3
+    a.pool[a.tables[0, j // 16], 1, which, 0, j % 16, 37] = 0xFF
+    a.call(**MANY)
+    torch.cuda.synchronize()
+    got = a.out.double().cpu()
+    clean = torch.ones_like(got, dtype=torch.bool)
+    if which == 0:
+        clean[25:28, :2] = False
+    else:
+        clean[25:28, :2, 37] = False
+    assert torch.isnan(got[~clean]).all()
+    bound = ref.attention_bound(want, weight, spread, floor, dh, a.out.dtype)
+    assert ((got - want).abs()[clean] <= bound[clean]).all()
+
+
+def test_many_rows_bad_blocks_contexts_and_starts():
+    a = Attention(17, 8, 2, 128, [(1, 64), (30, 70), (1, 30)])
+    want = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
+    a.tables[0, 1], a.tables[0, 2], a.ctx[0] = a.blocks, -1, 64 + 1600
+    a.call(**MANY)
+    torch.cuda.synchronize()
+    got = a.out.double().cpu()
+    bound = ref.attention_bound(*want, 128, a.out.dtype)
+    assert ((got - want[0]).abs()[1:] <= bound[1:]).all()
+    assert not torch.isnan(got).any() and int(a.err) == 1
+    for starts in ([0, 40, 2, 60], [0, 2, 40, 900], [0, -5, 2, 60], [3, 1, 2, 60]):
+        a = Attention(19, 8, 2, 64, [(20, 30), (20, 30), (20, 30)], pad=2)
+        a.starts = starts
+        a.call(**MANY)
+        torch.cuda.synchronize()
+        assert int(a.err) == 1
+
+
+def test_many_rows_large_and_small_scores():
+    for std in (200.0, 1e-6):
+        Attention(22, 8, 2, 128, [(30, 300), (1, 90)], q_std=std).check(**MANY)
+    for mag in (1e30, 1e-30):
+        a = Attention(24, 4, 2, 64, [(30, 200)])
+        a.q = (a.q.float() * mag).to(torch.bfloat16)
+        a.check(scale=float(0.125 / mag) if mag > 1 else 1e30, **MANY)
+
+
+def test_many_rows_captured_and_replayed_with_other_lengths():
+    a = Attention(25, 8, 2, 128, [(36, 500), (2, 90), (1, 333)])
+    a.call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        abi.attention_e4m3(a.q, a.out, a.pool, a.scales, a.layer, *a.d, a.ws, a.err, max_new=36)
+    for ctx in ([500, 90, 333], [100, 64, 3], [36, 2, 1]):
+        a.ctx = ctx
+        a.d[1].copy_(i32(ctx))
+        a.out.fill_(7.0)
+        want = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
+        g.replay()
+        torch.cuda.synchronize()
+        a.compare(*want)
+
+
+@pytest.mark.parametrize("dtype,max_new", [("bf16", 1), ("bf16", 6), ("bf16", 1000), ("f32", 6)])
+@pytest.mark.parametrize("times", [1000.0, 1e5])
+def test_attention_queries_with_an_element_far_above_the_rest(dtype, max_new, times):
+    """One dimension of the queries is `times` the others, and zero in every key: what counts are the small ones.
+    They are held to 2^-21 of their row's largest (bf16), which adds 2^-21 * max|q| * sum_d |K_jd| * scale to a score's
+    error; two f16 terms (fp32) hold them to 2^-22 of themselves and 2^-38 of the largest."""
+    a = Attention(27, 8, 2, 128, [(6, 300), (9, 90), (1, 40)], dtype)
+    a.q[:, :, 3] = a.q[:, :, 3].sign() * times
+    a.pool[:, :, 0, :, :, 3] = 0
+    want, weight, spread, floor = ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables)
+    k = ref.decode(a.pool[:, a.layer, 0].cpu(), a.scales[:, a.layer, 0].cpu()).abs().sum(-1).max()
+    unit = 2.0 ** -21 if dtype == "bf16" else 2.0 ** -38
+    extra = unit * a.q.double().cpu().abs().amax(-1) * k * 128 ** -0.5
+    a.call(max_new=max_new)
+    torch.cuda.synchronize()
+    a.compare(want, weight, spread + extra / ((128 + 8) * 2.0 ** -23), floor)
+
+
+# ---------------------------------------------------------------------------
 # Both, as a decoding step uses them.
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -1,5 +1,5 @@
 // yk_attention_e4m3.cu -- causal attention of a ragged batch over an e4m3 paged
-// KV cache (yk_attention_e4m3).
+// KV cache (yk_attention_e4m3): the kernel for fp32 queries, and the host side.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -25,6 +25,8 @@ namespace yk {
 //
 // Per page, with m16n8k16 f16 products and fp32 sums:
 //   S^T[16 keys x rows] = K Q^T, O^T[dims x rows] += V^T P^T.
+// Queries and weights are two f16 terms each, 22 bits: no floating-point input of
+// the matrix instructions has more than 11, and the e4m3 side is exact in f16.
 // Keys and dims are the products' M side, so 8 rows cost one n-tile: decoding
 // (4 or 8 rows) pays for 8, not 16 or 64.  e4m3 converts exactly to f16, and the
 // fragments come straight from 16-byte shared-memory reads: a product does not
@@ -37,43 +39,34 @@ namespace yk {
 // 2^(x + e_V - m), so that O needs no correction, and the sum adds p * 2^-e_V.
 // m follows the largest x + e_V of a row lazily: weights may exceed 1 by 2^8
 // before O is rescaled (their f16 form is biased by 2^7, the rest is room).
-// Queries go to f16 (fp32 queries and weights: to two f16 terms) after a shift of
-// each row by a power of two that brings its largest value next to 2^15.
+// Queries go to f16 terms after a shift of each row by a power of two that brings
+// its largest value next to 2^15.
 // ---------------------------------------------------------------------------
-constexpr int A8_THREADS = 128, A8_MAX_CTAS = 4;  // CTAs per SM at most
+constexpr int A8_THREADS = 128, A8_CTAS = 2;  // per SM
 
 // n-tiles of a warp at most: the O^T accumulators take 4 * DH / 16 registers each.
-template <typename AT, int DH>
+template <int DH>
 __host__ __device__ constexpr int a8_max_nt() {
-    return DH == 256 ? (sizeof(AT) == 4 ? 1 : 2) : (sizeof(AT) == 4 ? 2 : 4);
+    return DH == 256 ? 1 : 2;
 }
 
-// CTAs per SM, pages of a warp's share of the ring.
-template <typename AT, int DH, int NT>
-struct A8Shape {
-    static constexpr bool SMALL = sizeof(AT) == 2 && DH <= 128 && NT == 1;
-    static constexpr int CTAS = SMALL ? (DH == 64 ? 4 : 3) : 2;
-    static constexpr int DEPTH = SMALL ? (DH == 64 ? 4 : 3) : DH == 64 ? 8 : DH == 128 ? (NT == 4 ? 2 : 3) : 2;
-};
-
-template <typename AT, int DH, int NT>
+template <int DH, int NT>
 struct A8Cfg {
-    static constexpr int TERMS = sizeof(AT) == 4 ? 2 : 1;
+    static constexpr int TERMS = 2;  // of queries and weights
     static constexpr int KS = DH / 16, MT = DH / 16;  // k-steps of S^T, m-tiles of O^T
     static constexpr int ROWB = DH == 64 ? 64 : 128;  // bytes of a row in a TMA box
     static constexpr int BOX = 32 * ROWB;             // one box: 16 rows of K, 16 of V
     static constexpr int BOXES = DH / ROWB;
     static constexpr int PAGE = 32 * DH;
-    static constexpr int CTAS = A8Shape<AT, DH, NT>::CTAS, DEPTH = A8Shape<AT, DH, NT>::DEPTH;
+    static constexpr int DEPTH = DH == 64 ? 8 : DH == 128 ? 3 : 2;  // pages of a warp's share of the ring
     static constexpr int RING = 4 * DEPTH * PAGE;
-    static constexpr int CH = NT >= 3 ? 1 : 2;  // chains of score products
     static constexpr bool QREG = TERMS * NT * KS * 2 <= 48;  // queries in registers through the page loop
     static constexpr int ROWS = 8 * NT;                      // of a warp
     static constexpr int QBYTES = 2 * TERMS * NT * KS * 256;  // fragments of two row groups
     static constexpr int LDO = (DH < 128 ? DH : 128) + 4;    // floats of an accumulator row in shared memory
     static constexpr int DUMP = 4 * ROWS * LDO * 4;          // the warps' accumulators (128 dims at a time)
     // queries and accumulators share their room only where both do not fit beside the ring
-    static constexpr bool APART = CTAS * (RING + QBYTES + DUMP + 6144) <= 227 * 1024;
+    static constexpr bool APART = A8_CTAS * (RING + QBYTES + DUMP + 6144) <= 227 * 1024;
     static constexpr int QOFF = APART ? DUMP : 0;
     static constexpr int SHARED = APART ? QBYTES + DUMP : QBYTES > DUMP ? QBYTES : DUMP;
     static constexpr int NANS = 2 * ROWS * (DH / 32) * 4;    // bit per (row, dim)
@@ -115,10 +108,9 @@ __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m
         : "memory");
 }
 
-template <typename AT, int DH, int NT>
-__global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
-    attn8_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Attn8Params p) {
-    using C = A8Cfg<AT, DH, NT>;
+template <int DH, int NT>
+__global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Attn8Params p) {
+    using C = A8Cfg<DH, NT>;
     constexpr int TERMS = C::TERMS, KS = C::KS, MT = C::MT, NH = DH / 64;
     constexpr float LOWEST = -3.402823466e38f, LARGEST = 3.402823466e38f;
     extern __shared__ uint8_t smem_raw[];
@@ -250,11 +242,11 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
         fetch(1, bid2, gk2, kb2, vb2);
 
         // rows 8 u .. 8 u + 7 of a span's tile: lane's dims 64 h + 16 c .. + 15 of row 8 u + r
-        constexpr int QW = TERMS == 1 ? NH * 2 : NH * 4;
+        constexpr int QW = NH * 4;
         uint4 qw[QW];
         const auto load_q = [&](const Seg& sg, int u) {
             const int row = u * 8 + r, i = div_rep(p, sg.rem + row);
-            const AT* src = reinterpret_cast<const AT*>(p.q) + (size_t)(sg.tok + i) * p.q_stride +
+            const float* src = reinterpret_cast<const float*>(p.q) + (size_t)(sg.tok + i) * p.q_stride +
                             (size_t)(sg.g * rep + sg.rem + row - i * rep) * DH + 16 * c;
 #pragma unroll
             for (int h = 0; h < QW; ++h) {
@@ -263,8 +255,6 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                     qw[h] = __ldcg(reinterpret_cast<const uint4*>(src + 64 * (h / (QW / NH))) + h % (QW / NH));
             }
         };
-        if (TERMS == 1 && warp * 8 < segs[0].rows) load_q(segs[0], warp);
-
         int k = 0, issued = min(depth, nk);
 #pragma unroll 1
         for (int si = 0; si < nseg; ++si) {
@@ -280,20 +270,12 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
 #pragma unroll 1
             for (int u = warp; u * 8 < rows; u += 4) {
                 const int row = u * 8 + r;
-                if (u >= 4 || TERMS == 2) load_q(sg, u);
+                load_q(sg, u);
                 float amax = 0.f;
 #pragma unroll
-                for (int h = 0; h < QW; ++h) {
-                    if constexpr (TERMS == 1) {
-                        const uint32_t t[4] = {qw[h].x, qw[h].y, qw[h].z, qw[h].w};
-#pragma unroll
-                        for (int z = 0; z < 4; ++z)
-                            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(t[z] << 16)), fabsf(__uint_as_float(t[z] & 0xffff0000u))));
-                    } else {
-                        amax = fmaxf(fmaxf(fmaxf(amax, fabsf(__uint_as_float(qw[h].x))), fabsf(__uint_as_float(qw[h].y))),
-                                     fmaxf(fabsf(__uint_as_float(qw[h].z)), fabsf(__uint_as_float(qw[h].w))));
-                    }
-                }
+                for (int h = 0; h < QW; ++h)
+                    amax = fmaxf(fmaxf(fmaxf(amax, fabsf(__uint_as_float(qw[h].x))), fabsf(__uint_as_float(qw[h].y))),
+                                 fmaxf(fabsf(__uint_as_float(qw[h].z)), fabsf(__uint_as_float(qw[h].w))));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 // shift by 2^up: amax = m * 2^E, 1 <= m < 2, to m * 2^14
@@ -303,17 +285,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                 const uint32_t dst = smem_u32(shared + C::QOFF) + (uint32_t)(u * TERMS * KS * 256 + lane * 16);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    float x[4];
-                    if constexpr (TERMS == 1) {
-                        const uint32_t a = ks & 1 ? qw[ks >> 1].z : qw[ks >> 1].x, b = ks & 1 ? qw[ks >> 1].w : qw[ks >> 1].y;
-                        x[0] = __uint_as_float(a << 16);
-                        x[1] = __uint_as_float(a & 0xffff0000u);
-                        x[2] = __uint_as_float(b << 16);
-                        x[3] = __uint_as_float(b & 0xffff0000u);
-                    } else {
-                        x[0] = __uint_as_float(qw[ks].x); x[1] = __uint_as_float(qw[ks].y);
-                        x[2] = __uint_as_float(qw[ks].z); x[3] = __uint_as_float(qw[ks].w);
-                    }
+                    float x[4] = {__uint_as_float(qw[ks].x), __uint_as_float(qw[ks].y), __uint_as_float(qw[ks].z), __uint_as_float(qw[ks].w)};
 #pragma unroll
                     for (int z = 0; z < 4; ++z) x[z] *= f;
 #pragma unroll
@@ -323,10 +295,8 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                                          dst + (uint32_t)(t * KS * 256 + (ks >> 1) * 512 + (ks & 1) * 8)),
                                      "r"(y0), "r"(y1)
                                      : "memory");
-                        if (TERMS == 2) {  // what this term leaves
-                            const float2 a = f32x2(y0), b = f32x2(y1);
-                            x[0] -= a.x; x[1] -= a.y; x[2] -= b.x; x[3] -= b.y;
-                        }
+                        const float2 a = f32x2(y0), b = f32x2(y1);  // (what this term leaves)
+                        x[0] -= a.x; x[1] -= a.y; x[2] -= b.x; x[3] -= b.y;
                     }
                 }
             }
@@ -384,9 +354,9 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
             };
             float s[NT][4];
             const auto scores = [&]() {  // s = K Q^T of the page taken last
-                float s2[C::CH][NT][4];
+                float s2[2][NT][4];
 #pragma unroll
-                for (int ch = 0; ch < C::CH; ++ch)
+                for (int ch = 0; ch < 2; ++ch)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) s2[ch][nt][0] = s2[ch][nt][1] = s2[ch][nt][2] = s2[ch][nt][3] = 0.f;
 #pragma unroll
@@ -405,14 +375,14 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                                 const int at = ((nt * TERMS + t) * KS + h * 4 + i) / 2;
                                 const uint4 b = C::QREG ? qf[C::QREG ? at : 0] : lds128(q_smem + at * 512);
                                 mma_f16(s2[0][nt], a0, b.x, b.y);
-                                mma_f16(s2[C::CH - 1][nt], a1, b.z, b.w);
+                                mma_f16(s2[1][nt], a1, b.z, b.w);
                             }
                     }
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = C::CH == 2 ? s2[0][nt][i] + s2[C::CH - 1][nt][i] : s2[0][nt][i];
+                    for (int i = 0; i < 4; ++i) s[nt][i] = s2[0][nt][i] + s2[1][nt][i];
             };
             if (k < k_end) {
                 take(k);
@@ -491,10 +461,8 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                         for (int j = 0; j < 2; ++j) {
                             const uint32_t x = pack_f16(s[nt][2 * j], s[nt][2 * j + 1]);
                             pb[0][nt][j] = transpose8(x);
-                            if constexpr (TERMS == 2) {
-                                const float2 a = f32x2(x);
-                                pb[TERMS - 1][nt][j] = transpose8(pack_f16(s[nt][2 * j] - a.x, s[nt][2 * j + 1] - a.y));
-                            }
+                            const float2 a = f32x2(x);
+                            pb[1][nt][j] = transpose8(pack_f16(s[nt][2 * j] - a.x, s[nt][2 * j + 1] - a.y));
                         }
                     }
                 }
@@ -579,8 +547,6 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
             }
 
             // ---- end of the span: the parts of a row group are joined in shared memory
-            // (the next span's queries come meanwhile)
-            if (TERMS == 1 && si + 1 < nseg && warp * 8 < segs[si + 1].rows) load_q(segs[si + 1], warp);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -649,7 +615,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
                     if (whole) {
                         const float z = L == 0.f ? 0.f : 1.0f / L;
                         const int tok = row_token(row);
-                        store4(reinterpret_cast<AT*>(p.out) + (size_t)(sg.tok + tok) * p.out_stride +
+                        store4(reinterpret_cast<float*>(p.out) + (size_t)(sg.tok + tok) * p.out_stride +
                                    (size_t)(sg.g * rep + sg.rem + row - tok * rep) * DH + d, a.x * z, a.y * z, a.z * z, a.w * z);
                     } else {
                         __stcg(reinterpret_cast<float4*>(p.ws_o + (part_row + row) * DH + d), a);
@@ -669,7 +635,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8Shape<AT, DH, NT>::CTAS)
         }
         __syncthreads();  // (the span list too)
     }
-    a8_join<AT, DH, A8_THREADS>(p, R, rep, s_last, s_cut);
+    a8_join<float, DH, A8_THREADS>(p, R, rep, s_last, s_cut);
     // every copy asked for has landed: the loop above waited for each, unless it gave up
     if (dead && rg == 0 && lane == 0)
         for (int i = 0; i < depth; ++i)
@@ -753,44 +719,40 @@ yk_status attention_e4m3_check(const yk_attention_e4m3_args& a) {
     return YK_OK;
 }
 
-template <typename AT, int DH, int NT>
+template <int DH, int NT>
 static yk_status launch_a8(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, const Attn8Params& p) {
-    using C = A8Cfg<AT, DH, NT>;
-    static_assert(C::CTAS <= A8_MAX_CTAS && C::CTAS * C::ROWS * (2 * NT > a8_max_nt<AT, DH>() ? 2 : 1) <= A8_WS / DH,
+    using C = A8Cfg<DH, NT>;
+    static_assert(A8_CTAS * C::ROWS * (2 * NT > a8_max_nt<DH>() ? 2 : 1) <= A8_WS / DH,
                   "cut spans' rows in the workspace");
     int dev = 0;
     YK_CHECK_CUDA(cudaGetDevice(&dev));
     static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
     const uint64_t bit = 1ull << (dev & 63);
     if (!(ready.load(std::memory_order_acquire) & bit)) {
-        YK_CHECK_CUDA(cudaFuncSetAttribute(attn8_kernel<AT, DH, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
+        YK_CHECK_CUDA(cudaFuncSetAttribute(attn8_kernel<DH, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM));
         ready.fetch_or(bit, std::memory_order_release);
     }
-    YK_CHECK_CUDA(launch_on(st, pdl, attn8_kernel<AT, DH, NT>, num_sms * C::CTAS, A8_THREADS, C::SMEM, map, p));
+    YK_CHECK_CUDA(launch_on(st, pdl, attn8_kernel<DH, NT>, num_sms * A8_CTAS, A8_THREADS, C::SMEM, map, p));
     return YK_OK;
 }
 
 // The tile: as few n-tiles as hold the rows of a sequence's new tokens; beyond a
 // warp's most, two row groups share the pages.
-template <typename AT, int DH>
+template <int DH>
 static yk_status launch_a8_rows(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, Attn8Params& p,
                                 long long rows) {
-    constexpr int MOST = a8_max_nt<AT, DH>();
+    constexpr int MOST = a8_max_nt<DH>();
     p.lg = rows > 8 * MOST ? 1 : 0;
     const int nt = (int)std::min<long long>(MOST, (rows + (8 << p.lg) - 1) / (8 << p.lg));
-    if constexpr (MOST >= 4) {
-        if (nt == 4) return launch_a8<AT, DH, 4>(st, pdl, num_sms, map, p);
-        if (nt == 3) return launch_a8<AT, DH, 3>(st, pdl, num_sms, map, p);
-    }
     if constexpr (MOST >= 2) {
-        if (nt == 2) return launch_a8<AT, DH, 2>(st, pdl, num_sms, map, p);
+        if (nt == 2) return launch_a8<DH, 2>(st, pdl, num_sms, map, p);
     }
-    return launch_a8<AT, DH, 1>(st, pdl, num_sms, map, p);
+    return launch_a8<DH, 1>(st, pdl, num_sms, map, p);
 }
 
 yk_status attention_e4m3_launch(cudaStream_t st, bool pdl, int num_sms, const yk_attention_e4m3_args& a) {
     if (a.T == 0) return YK_OK;
-    YK_ARG(num_sms * A8_MAX_CTAS * 4 <= A8_COUNTERS, "device has more SMs than the workspace's counters");
+    YK_ARG(num_sms * A8_CTAS * 4 <= A8_COUNTERS, "device has more SMs than the workspace's counters");
     CUtensorMap map;
     YK_TRY(page_map(a.pages, a.dtype == YK_DTYPE_F32, &map));
     Attn8Params p;
@@ -833,9 +795,9 @@ yk_status attention_e4m3_launch(cudaStream_t st, bool pdl, int num_sms, const yk
     const long long rows = most * (a.n_heads / a.pages.n_kv_heads);
     if (a.dtype == YK_DTYPE_BF16) return attention_e4m3_launch_bf16(st, pdl, num_sms, dh, map, p, rows);
     switch (dh) {
-        case 64: return launch_a8_rows<float, 64>(st, pdl, num_sms, map, p, rows);
-        case 128: return launch_a8_rows<float, 128>(st, pdl, num_sms, map, p, rows);
-        default: return launch_a8_rows<float, 256>(st, pdl, num_sms, map, p, rows);
+        case 64: return launch_a8_rows<64>(st, pdl, num_sms, map, p, rows);
+        case 128: return launch_a8_rows<128>(st, pdl, num_sms, map, p, rows);
+        default: return launch_a8_rows<256>(st, pdl, num_sms, map, p, rows);
     }
 }
 

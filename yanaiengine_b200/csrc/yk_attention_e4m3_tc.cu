@@ -582,19 +582,22 @@ static yk_status launch_tca(cudaStream_t st, bool pdl, int num_sms, const CUtens
 }
 
 // rows: (token, head) rows of a sequence's new tokens, as far as the caller says.
-// The tile holds them all up to 64 (head_dim 256: 16), rounded up to the next shape.
+// The tile holds them all up to 48 (head_dim 64: 32, head_dim 256: 16), rounded up
+// to the next shape; beyond, the kernel for many rows takes over.  16 sequences of
+// 500 to 3000 keys, 8 KV heads, this kernel and the other: head_dim 128, 40 rows 43
+// and 45 us, 48 rows 46 and 45, 64 rows 58 and 49; head_dim 64, 32 rows 32 and 33,
+// 40 rows 38 and 33, 64 rows 48 and 34.  (The other has no room for head_dim 256.)
 template <int DH>
 static yk_status launch_tca_rows(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, const Attn8Params& p,
                                  long long rows) {
-    if (DH != 256 && rows > 64) return attention_e4m3_launch_rows(st, pdl, num_sms, DH, map, p);
+    if (DH != 256 && rows > (DH == 64 ? 32 : 48)) return attention_e4m3_launch_rows(st, pdl, num_sms, DH, map, p);
     if (rows <= 8) return launch_tca<DH, 1>(st, pdl, num_sms, map, p);
     if (DH == 256 || rows <= 16) return launch_tca<DH, 2>(st, pdl, num_sms, map, p);
     if constexpr (DH != 256) {
         if (rows <= 24) return launch_tca<DH, 3>(st, pdl, num_sms, map, p);
         if (rows <= 32) return launch_tca<DH, 4>(st, pdl, num_sms, map, p);
-        if (rows <= 48) return launch_tca<DH, 6>(st, pdl, num_sms, map, p);
-        return launch_tca<DH, 8>(st, pdl, num_sms, map, p);
     }
+    if constexpr (DH == 128) return launch_tca<DH, 6>(st, pdl, num_sms, map, p);
     return YK_OK;
 }
 
