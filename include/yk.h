@@ -364,7 +364,13 @@ yk_status yk_kv_append(int32_t device, void* stream, const yk_kv_append_args* ar
  * aligned), both F32 or both BF16.
  * workspace: yk_attention_e4m3_workspace bytes, 16-byte aligned, zeroed once by
  * the caller before its first use; every call leaves it ready for the next.
- * Calls that overlap on the GPU need a workspace each. */
+ * Calls that overlap on the GPU need a workspace each.
+ * Scores, sums and results are fp32 inside.  Weights are rounded to 11 bits (F32:
+ * 22) and count as nothing from 2^-28 (2^-32) of their row's largest down; queries
+ * are held to 2^-21 of their row's largest value (F32: to 22 bits).
+ * At most 1024 query heads to a KV head and 2^25 columns of block_tables;
+ * YK_ERR_UNSUPPORTED from T * n_heads or (T * n_heads / 8 + B * n_kv_heads) *
+ * max_blocks = 2^31 on: split the batch. */
 typedef struct yk_attention_e4m3_args {
     yk_kv_pages    pages;
     int32_t        layer;
