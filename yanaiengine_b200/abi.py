@@ -329,35 +329,36 @@ def tp_unique_id() -> bytes:
 _APPEND = struct.Struct("@2P5i4x5ifPqPq5P")
 _ATTENTION = struct.Struct("@2P5i4x8i2fPqPq4PQP")
 assert _APPEND.size == C.sizeof(KVAppendArgs) and _ATTENTION.size == C.sizeof(AttentionE4M3Args)
-_INTS, _FLOATS = frozenset(("torch.int32", "torch.uint32")), {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16}
-_dtypes: dict = {}  # torch dtype -> (name, element size)
+_dtypes: dict = {}  # torch dtype -> (KV_* of cells of it, YK_DTYPE_* or None, 32-bit integer)
 
 
-def _kind(t):
-    d = t.dtype
-    k = _dtypes.get(d)
-    if k is None:
-        k = _dtypes[d] = (str(d), t.element_size())
-    return k
+def _type(d):
+    import torch
+
+    size = torch.empty(0, dtype=d).element_size()
+    code = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}.get(d)
+    kind = KV_E4M3 if size == 1 else {DTYPE_F32: KV_F32, DTYPE_BF16: KV_BF16, None: None}[code]
+    r = _dtypes[d] = (kind, code, d in (torch.int32, torch.uint32))
+    return r
 
 
 def _code(t, name: str) -> int:
-    c = _FLOATS.get(_kind(t)[0])
+    c = (_dtypes.get(t.dtype) or _type(t.dtype))[1]
     if c is None:
         raise ValueError(f"{name}: float32 or bfloat16, not {t.dtype}")
     return c
 
 
 def _ints(t, name: str, device: int, numel: int = -1) -> int:
-    if t.get_device() != device or not t.is_contiguous() or _kind(t)[0] not in _INTS or 0 <= numel != t.numel():
+    if (t.get_device() != device or not t.is_contiguous() or not (_dtypes.get(t.dtype) or _type(t.dtype))[2] or
+            0 <= numel and 4 * numel != t.nbytes):
         raise ValueError(f"{name} must be contiguous 32-bit integers on cuda:{device}" + (f", {numel} of them" if numel >= 0 else ""))
     return t.data_ptr()
 
 
 def _reals(t, name: str, device: int, numel: int) -> int:
-    if t is None:
-        return 0
-    if t.get_device() != device or not t.is_contiguous() or _kind(t)[0] != "torch.float32" or numel != t.numel():
+    if (t.get_device() != device or 4 * numel != t.nbytes or not t.is_contiguous() or
+            (_dtypes.get(t.dtype) or _type(t.dtype))[1] != DTYPE_F32):
         raise ValueError(f"{name} must be {numel} contiguous float32 values on cuda:{device}")
     return t.data_ptr()
 
@@ -365,43 +366,44 @@ def _reals(t, name: str, device: int, numel: int) -> int:
 def _pages(pool, scales, device: int) -> tuple:
     """The fields of yk_kv_pages.  pool [blocks, layers, 2, kv heads, 16, head_dim]: 1-byte elements with scales
     [blocks, layers, 2, kv heads] (1-byte elements), or fp32 / bf16 and scales None."""
-    if pool.dim() != 6:
+    shape = pool.shape
+    if len(shape) != 6 or shape[2] != 2 or shape[4] != BLOCK_SIZE:
         raise ValueError("pool must be [blocks, layers, 2, kv heads, 16, head_dim]")
-    n, layers, two, g, slots, dh = pool.shape
-    if two != 2 or slots != BLOCK_SIZE:
-        raise ValueError("pool must be [blocks, layers, 2, kv heads, 16, head_dim]")
-    if pool.get_device() != device or device < 0 or not pool.is_contiguous():
+    n, layers, _, g, _, dh = shape
+    if device < 0 or pool.get_device() != device or not pool.is_contiguous():
         raise ValueError(f"pool is not on cuda:{device}, or not contiguous")
-    if _kind(pool)[1] != 1:
+    kind = (_dtypes.get(pool.dtype) or _type(pool.dtype))[0]
+    if kind != KV_E4M3:
+        if kind is None:
+            raise ValueError(f"pool: float32, bfloat16 or bytes, not {pool.dtype}")
         if scales is not None:
             raise ValueError("scales belong to a pool of 8-bit cells")
-        return pool.data_ptr(), 0, KV_F32 if _code(pool, "pool") == DTYPE_F32 else KV_BF16, n, layers, g, dh
+        return pool.data_ptr(), 0, kind, n, layers, g, dh
     if scales is None:
         raise ValueError("a pool of 8-bit cells needs scales")
-    if scales.get_device() != device or not scales.is_contiguous() or _kind(scales)[1] != 1 or scales.numel() != n * layers * 2 * g:
+    if (scales.get_device() != device or scales.nbytes != n * layers * 2 * g or not scales.is_contiguous() or
+            (_dtypes.get(scales.dtype) or _type(scales.dtype))[0] != KV_E4M3):
         raise ValueError(f"scales must be [blocks, layers, 2, kv heads] contiguous bytes on cuda:{device}")
-    return pool.data_ptr(), scales.data_ptr(), KV_E4M3, n, layers, g, dh
+    return pool.data_ptr(), scales.data_ptr(), kind, n, layers, g, dh
 
 
 def _rows(t, name: str, device: int, tokens: int, heads: int, dh: int) -> tuple:
     """(address, elements between tokens) of [tokens, heads, head_dim] (or [tokens, heads * head_dim])."""
-    s, shape = t.stride(), t.shape
-    if len(s) == 3:
-        good = s[1] == dh and s[2] == 1 and shape[1] == heads and shape[2] == dh
-    else:
-        good = len(s) == 2 and s[1] == 1 and shape[1] == heads * dh
-    if not good or shape[0] != tokens or t.get_device() != device:
-        raise ValueError(f"{name} must be [{tokens}, {heads}, {dh}] on cuda:{device}, its rows contiguous")
-    return t.data_ptr(), (s[0] if tokens > 1 else heads * dh)
+    shape, row = t.shape, heads * dh
+    if (shape == (tokens, heads, dh) or shape == (tokens, row)) and t.get_device() == device:
+        if t.is_contiguous():
+            return t.data_ptr(), row
+        s = t.stride()
+        if s[-1] == 1 and (len(s) == 2 or s[1] == dh):
+            return t.data_ptr(), (s[0] if tokens > 1 else row)
+    raise ValueError(f"{name} must be [{tokens}, {heads}, {dh}] on cuda:{device}, its rows contiguous")
 
 
 _raw_stream = None
 
 
-def _stream(device: int, stream):
+def _current_stream(device: int) -> int:
     global _raw_stream
-    if stream is not None:
-        return stream
     if _raw_stream is None:
         import torch
 
@@ -416,13 +418,16 @@ def kv_append(pool, scales, layer: int, qkv, q_out, slots, rope, q_gain, k_gain,
     queries to q_out [T, heads, head_dim], keys and values to cache slots [T] (int32) of `layer`.
     rope [T, head_dim / 2, 2], q_gain / k_gain [head_dim]: fp32 or None; err: int32 [1] or None."""
     dev = qkv.get_device()
-    pages = _pages(pool, scales, dev)
-    g, dh, n = pages[5], pages[6], slots.numel()
-    a = _APPEND.pack(*pages, layer, n, heads, _code(qkv, "qkv"), _code(q_out, "q_out"), eps,
-                     *_rows(qkv, "qkv", dev, n, heads + 2 * g, dh), *_rows(q_out, "q_out", dev, n, heads, dh),
-                     _ints(slots, "slots", dev), _reals(rope, "rope", dev, n * dh), _reals(q_gain, "q_gain", dev, dh),
-                     _reals(k_gain, "k_gain", dev, dh), 0 if err is None else _ints(err, "err", dev))
-    st = lib().yk_kv_append(dev, _stream(dev, stream), a)
+    data, scale, kind, blocks, layers, g, dh = _pages(pool, scales, dev)
+    n = slots.numel()
+    src, src_stride = _rows(qkv, "qkv", dev, n, heads + 2 * g, dh)
+    dst, dst_stride = _rows(q_out, "q_out", dev, n, heads, dh)
+    a = _APPEND.pack(data, scale, kind, blocks, layers, g, dh, layer, n, heads, _code(qkv, "qkv"), _code(q_out, "q_out"), eps,
+                     src, src_stride, dst, dst_stride, _ints(slots, "slots", dev),
+                     0 if rope is None else _reals(rope, "rope", dev, n * dh),
+                     0 if q_gain is None else _reals(q_gain, "q_gain", dev, dh),
+                     0 if k_gain is None else _reals(k_gain, "k_gain", dev, dh), 0 if err is None else _ints(err, "err", dev))
+    st = (_lib or lib()).yk_kv_append(dev, _current_stream(dev) if stream is None else stream, a)
     if st:
         check(st)
 
@@ -433,21 +438,23 @@ def attention_e4m3(q, out, pool, scales, layer: int, q_starts, context_lens, blo
     q_starts [B + 1], context_lens [B], block_tables [B, max_blocks]: int32; workspace: bytes (at least
     attention_e4m3_workspace(...)), zeroed once by the caller; err: int32 [1] or None."""
     dev = q.get_device()
-    pages = _pages(pool, scales, dev)
-    if q.dim() != 3 or block_tables.dim() != 2:
+    data, scales_at, kind, blocks, layers, g, dh = _pages(pool, scales, dev)
+    shape, table = q.shape, block_tables.shape
+    if len(shape) != 3 or len(table) != 2:
         raise ValueError("q must be [T, heads, head_dim], block_tables [B, max_blocks]")
-    n, heads, dh = q.shape
-    B, width = block_tables.shape
-    if dh != pages[6] or out.dtype != q.dtype:
+    n, heads, width = shape
+    B, columns = table
+    if width != dh or out.dtype != q.dtype:
         raise ValueError("q, out and the pool disagree on head_dim or dtype")
     if workspace.get_device() != dev or not workspace.is_contiguous():
         raise ValueError(f"workspace must be contiguous on cuda:{dev}")
-    a = _ATTENTION.pack(*pages, layer, n, B, heads, _code(q, "q"), width, max_new, window, scale, cap,
-                        *_rows(q, "q", dev, n, heads, dh), *_rows(out, "out", dev, n, heads, dh),
-                        _ints(q_starts, "q_starts", dev, B + 1), _ints(context_lens, "context_lens", dev, B),
-                        _ints(block_tables, "block_tables", dev), workspace.data_ptr(), workspace.nbytes,
-                        0 if err is None else _ints(err, "err", dev))
-    st = lib().yk_attention_e4m3(dev, _stream(dev, stream), a)
+    q_at, q_stride = _rows(q, "q", dev, n, heads, dh)
+    out_at, out_stride = _rows(out, "out", dev, n, heads, dh)
+    a = _ATTENTION.pack(data, scales_at, kind, blocks, layers, g, dh, layer, n, B, heads, _code(q, "q"), columns, max_new, window,
+                        scale, cap, q_at, q_stride, out_at, out_stride, _ints(q_starts, "q_starts", dev, B + 1),
+                        _ints(context_lens, "context_lens", dev, B), _ints(block_tables, "block_tables", dev),
+                        workspace.data_ptr(), workspace.nbytes, 0 if err is None else _ints(err, "err", dev))
+    st = (_lib or lib()).yk_attention_e4m3(dev, _current_stream(dev) if stream is None else stream, a)
     if st:
         check(st)
 

@@ -459,6 +459,9 @@ static yk_status device_sms(int32_t device, const char* what, int* sms) {
     return YK_OK;
 }
 
+// The operators' launches may begin before the kernel ahead of them in the stream
+// has ended: they wait for its end (griddepcontrol.wait) before they touch memory,
+// whatever kernel it is.
 // Runs body(SMs of `device`) with `device` current; a CUDA error that earlier work
 // left pending on this thread is returned before anything is launched.
 template <typename F>
@@ -484,7 +487,7 @@ extern "C" yk_status yk_kv_append(int32_t device, void* stream, const yk_kv_appe
     YK_ARG(args, "args is null");
     YK_TRY(yk::kv_append_check(*args));
     return yk::on_device(device, "yk_kv_append", [&](int sms) {
-        return yk::kv_append_launch(static_cast<cudaStream_t>(stream), false, sms, *args);
+        return yk::kv_append_launch(static_cast<cudaStream_t>(stream), true, sms, *args);
     });
 }
 
@@ -503,6 +506,6 @@ extern "C" yk_status yk_attention_e4m3(int32_t device, void* stream, const yk_at
     return yk::on_device(device, "yk_attention_e4m3", [&](int sms) -> yk_status {
         YK_ARG(args->T == 0 || args->workspace_bytes >= yk::attention_e4m3_ws_bytes(sms, args->pages.head_dim),
                "workspace_bytes is below yk_attention_e4m3_workspace's");
-        return yk::attention_e4m3_launch(static_cast<cudaStream_t>(stream), false, sms, *args);
+        return yk::attention_e4m3_launch(static_cast<cudaStream_t>(stream), true, sms, *args);
     });
 }
