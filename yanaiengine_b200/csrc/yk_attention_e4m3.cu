@@ -45,6 +45,7 @@ namespace yk {
 // its largest value next to 2^15.
 // ---------------------------------------------------------------------------
 constexpr int A8_THREADS = 128, A8_CTAS = 2;  // per SM
+constexpr int A8_COST = 8;                    // a span's own cost, in pages
 
 // n-tiles of a warp at most: the O^T accumulators take 4 * DH / 16 registers each.
 template <int DH>
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
     pdl_wait();
 
     A8Work work;
-    if (!a8_plan<A8_THREADS, 1, 0>(p, R, rep, s_scan, work)) return;
+    if (!a8_plan<A8_THREADS, 1, A8_COST, 8>(p, R, rep, s_scan, work)) return;
 
     // per-thread places in a page: K rows sigma(r), sigma(r) + 8; V rows c, c + 4, c + 8, c + 12
     const int sigma = (r & 1) * 4 + (r >> 1);
@@ -179,9 +180,15 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
     int in_slot = 0, in_phase = 1, out_slot = 0, out_phase = 0;  // of the ring: next to fill, next to read
     // the spans of this CTA's range, A8_SEGS of them at a time
     for (int seg0 = 0; seg0 < work.nspans; seg0 += A8_SEGS) {
-        a8_list<1, 0>(p, R, rep, work, seg0, segs);
+        a8_list<1, A8_COST>(p, R, rep, work, seg0, segs);
         __syncthreads();
         const int nseg = min(A8_SEGS, work.nspans - seg0);
+        if (threadIdx.x == 0)
+            for (int i = 0, at = 0; i < nseg; ++i) {
+                segs[i].v = at;
+                at += segs[i].n;
+            }
+        __syncthreads();
         const int v0 = segs[0].v, v1 = segs[nseg - 1].v + segs[nseg - 1].n;
         const int nk = (v1 - v0 - part + nparts - 1) / nparts;  // pages of this part
 

@@ -9,7 +9,6 @@ namespace yk {
 
 constexpr int A8_SEGS = 32;        // spans a CTA lists at a time
 constexpr int A8_COUNTERS = 4096;  // bytes of arrival counters, one per CTA
-constexpr int A8_MIN_PAGES = 8;    // pages of a CTA's range, at least
 constexpr int A8_SCAN = 48;        // shared words of a8_plan
 constexpr float A8_LOWEST = -3.402823466e38f, A8_LARGEST = 3.402823466e38f;
 
@@ -38,7 +37,7 @@ struct Seg {
     int rows;
     int pos;         // position of that token
     int page, pend;  // first page of this CTA's part; pages of the span's keys end here
-    int v, n;        // its place and length (pages) in the CTA's range
+    int v, n;        // its place among the listed spans' units (the kernel's own affair) and its length
     int c0, c1;      // first and last CTA of the span
 };
 
@@ -94,7 +93,7 @@ __device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& star
 }
 
 
-// A thread's sequences and this CTA's range of units, [lo, hi) of the spans laid end to end.  A span has COST units
+// A thread's sequences and this CTA's range of units (LEAST at least), [lo, hi) of the spans laid end to end.  A span has COST units
 // more than its pages fill, in front, for what it costs beside them: spans that come and go quickly count.
 struct A8Work {
     int b_lo, b_hi;
@@ -108,7 +107,7 @@ struct A8Work {
 
 // Block-wide: the range from the lengths on the device (prefix sums over the
 // sequences, THREADS threads).  False: nothing for this CTA.
-template <int THREADS, int PU, int COST>
+template <int THREADS, int PU, int COST, int LEAST>
 __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, unsigned* s_scan, A8Work& w) {
     constexpr int WARPS = THREADS / 32;
     static_assert(2 * WARPS + 2 <= A8_SCAN, "scan words");
@@ -159,7 +158,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     const unsigned total = __reduce_add_sync(0xffffffffu, wu);
     w.at0 += __reduce_add_sync(0xffffffffu, lane < warp ? wu : 0u) - w.units;
     w.ord0 += (int)__reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u) - spans;
-    w.per = max((unsigned)(A8_MIN_PAGES / PU), (total + gridDim.x - 1) / gridDim.x);
+    w.per = max((unsigned)LEAST, (total + gridDim.x - 1) / gridDim.x);
     w.lo = min(total, blockIdx.x * w.per);
     w.hi = min(total, w.lo + w.per);
     if (w.lo >= w.hi) return false;
@@ -228,7 +227,7 @@ __device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, co
                     x.pos = ctx - n + s.tok;
                     x.page = s.page + PU * (int)(max(from, w.lo) - from);
                     x.pend = s.pend;
-                    x.v = (int)(max(from, w.lo) - w.lo);
+                    x.v = 0;
                     x.n = (int)(min(to, w.hi) - max(from, w.lo));
                     x.c0 = x.c1 = (int)blockIdx.x;
                     if (from < w.lo) x.c0 -= (int)((w.lo - from + w.per - 1) / w.per);

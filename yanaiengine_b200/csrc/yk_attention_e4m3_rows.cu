@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
     pdl_wait();
     A8Work work;
     if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
-    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
+    const bool busy = a8_plan<TCR_THREADS, TCA_PAGES, TCA_COST, 1>(p, R, rep, s_scan, work);  // (block-uniform)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

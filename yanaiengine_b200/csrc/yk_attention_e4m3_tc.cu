@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
     pdl_wait();
     A8Work work;
     if (warp == 14) tmem_alloc(smem_u32(s_tmem), C::TMEM);
-    const bool busy = a8_plan<TCA_THREADS, TCA_PAGES, TCA_COST>(p, R, rep, s_scan, work);  // (block-uniform)
+    const bool busy = a8_plan<TCA_THREADS, TCA_PAGES, TCA_COST, 1>(p, R, rep, s_scan, work);  // (block-uniform)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -601,7 +601,8 @@ static yk_status launch_tca_rows(cudaStream_t st, bool pdl, int num_sms, const C
                                  long long rows) {
     if (DH != 256 && rows > (DH == 64 ? 32 : 48)) return attention_e4m3_launch_rows(st, pdl, num_sms, DH, map, p);
     if (rows <= 8) return launch_tca<DH, 1>(st, pdl, num_sms, map, p);
-    if (DH == 256 || rows <= 16) return launch_tca<DH, 2>(st, pdl, num_sms, map, p);
+    if (rows <= 16) return launch_tca<DH, 2>(st, pdl, num_sms, map, p);
+    if constexpr (DH == 256) return launch_tca<DH, 4>(st, pdl, num_sms, map, p);
     if constexpr (DH != 256) {
         if (rows <= 24) return launch_tca<DH, 3>(st, pdl, num_sms, map, p);
         if (rows <= 32) return launch_tca<DH, 4>(st, pdl, num_sms, map, p);
