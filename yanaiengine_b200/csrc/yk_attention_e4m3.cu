@@ -39,13 +39,13 @@ namespace yk {
 // 2^(x + e_V - m), so that O needs no correction, and the sum adds p * 2^-e_V.
 // m follows the largest x + e_V of a row lazily: weights may exceed 1 by 2^8
 // before O is rescaled (their f16 form is biased by 2^7, the rest is room).
-// Measured: 9 sequences of 300-1900 keys, 5 tokens, 12 heads of 64, window 333: 15
+// Measured: 9 sequences of 300-1900 keys, 5 tokens, 12 heads of 64, window 333: 11
 // us, nearly all of it latency (launch, plan, first pages, join).
 // Queries go to f16 terms after a shift of each row by a power of two that brings
 // its largest value next to 2^15.
 // ---------------------------------------------------------------------------
 constexpr int A8_THREADS = 128, A8_CTAS = 2;  // per SM
-constexpr int A8_COST = 8;                    // a span's own cost, in pages
+constexpr int A8_COST = 8;                    // a span's own cost, in pages (11 sequences of 3 tokens: 23.9 -> 6.7 us, 16 of 500-2500 keys: 31.5 -> 28.6)
 
 // n-tiles of a warp at most: the O^T accumulators take 4 * DH / 16 registers each.
 template <int DH>

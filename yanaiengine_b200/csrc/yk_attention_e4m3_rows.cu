@@ -187,6 +187,10 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
         a8_list<TCA_PAGES, TCA_COST>(p, R, rep, work, seg0, segs);
         __syncthreads();
         const int nseg = min(A8_SEGS, work.nspans - seg0);
+        // Queries of 128 rows are 32 steps of one warp, about 8 tiles' time: behind a shorter span the V warps convert
+        // their share while it begins (200 tokens over 2000 keys: 48 -> 31 us; done for every span, the long
+        // prompts lose 6 %).
+        const auto shared_queries = [&](int si) { return si == 0 || segs[si - 1].n < 8; };
         if (warp < 8) {
             // ---------------- softmax: row 32 * quad + lane; group 0 takes the even tiles, group 1 the odd ones ----------------
             const int quad = warp & 3, group = warp >> 2, row = 32 * quad + lane;
@@ -309,11 +313,16 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
             // ---------------- V: e4m3 -> f16, and the results ----------------
             const int tid = threadIdx.x - 256, quad = warp & 3;
             const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-            if (seg0 == 0) {
-                convert_queries<DH, R, true>(p, segs[0], rep, lane, quad, 5, s_q, s_rf, [] { return true; });
-                fence_proxy_async_smem();
-                first_queries_bar();
-            }
+            const auto queries = [&](int si) {
+                if (shared_queries(si)) {
+                    convert_queries<DH, R, true>(p, segs[si], rep, lane, quad, 5, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
+                                                 [&] { wait(q_empty + 8 * qt.slot, qt.phase ^ 1); return !dead; });
+                    fence_proxy_async_smem();
+                    queries_bar();
+                }
+                qt.next();
+            };
+            queries(0);
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
                 const Seg sg = segs[si];
@@ -333,6 +342,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                     }
                     vt.next();
                     wt.next();
+                    if (i == 0 && si + 1 < nseg) queries(si + 1);
                 }
                 // ---- the span's result: this thread's row is tid
                 const bool whole = sg.c0 == sg.c1, mine = tid < sg.rows;
@@ -425,6 +435,9 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
                 const int n = segs[si].n;
+                // (queries come from the V warps too, which first write the results before them: nothing may wait here for those)
+                if (!__all_sync(0xffffffffu, mbar_test(q_full + 8 * qt.slot, (uint32_t)qt.phase)))
+                    while (pending > 0) values();
                 wait(q_full + 8 * qt.slot, qt.phase);
 #pragma unroll 1
                 for (int i = 0; i < n; ++i) {
@@ -458,11 +471,11 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
             // ---------------- queries: two terms of each row ----------------
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
-                const bool first = seg0 + si == 0;
-                convert_queries<DH, R, true>(p, segs[si], rep, lane, first ? 4 : 0, first ? 5 : 1, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
+                const bool shared = shared_queries(si);
+                convert_queries<DH, R, true>(p, segs[si], rep, lane, shared ? 4 : 0, shared ? 5 : 1, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
                                              [&] { wait(q_empty + 8 * qt.slot, qt.phase ^ 1); return !dead; });
                 fence_proxy_async_smem();
-                if (first) first_queries_bar();
+                if (shared) queries_bar();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full + 8 * qt.slot);
                 qt.next();

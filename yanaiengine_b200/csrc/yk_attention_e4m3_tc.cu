@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
             if (seg0 == 0 && RN > 1) {
                 convert_queries<DH, R, C::JOINED>(p, segs[0], rep, lane, quad, 5, s_q, s_rf, [] { return true; });
                 fence_proxy_async_smem();
-                first_queries_bar();
+                queries_bar();
             }
 #pragma unroll 1
             for (int si = 0; si < nseg; ++si) {
@@ -551,7 +551,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                 convert_queries<DH, R, C::JOINED>(p, segs[si], rep, lane, first ? 4 : 0, first ? 5 : 1, s_q + qt.slot * C::QB, s_rf + qt.slot * R,
                                              [&] { wait(q_empty + 8 * qt.slot, qt.phase ^ 1); return !dead; });
                 fence_proxy_async_smem();
-                if (first) first_queries_bar();
+                if (first) queries_bar();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full + 8 * qt.slot);
                 qt.next();
@@ -591,11 +591,13 @@ static yk_status launch_tca(cudaStream_t st, bool pdl, int num_sms, const CUtens
 }
 
 // rows: (token, head) rows of a sequence's new tokens, as far as the caller says.
-// The tile holds them all up to 48 (head_dim 64: 32, head_dim 256: 16), rounded up
+// The tile holds them all up to 48 (head_dim 64 and 256: 32), rounded up
 // to the next shape; beyond, the kernel for many rows takes over.  16 sequences of
 // 500 to 3000 keys, 8 KV heads, this kernel and the other: head_dim 128, 40 rows 43
 // and 45 us, 48 rows 46 and 45, 64 rows 58 and 49; head_dim 64, 32 rows 32 and 33,
-// 40 rows 38 and 33, 64 rows 48 and 34.  (The other has no room for head_dim 256.)
+// 40 rows 38 and 33, 64 rows 48 and 34.  (The other has no room for head_dim 256, whose
+// prompts take tiles of 32 rows: 700 tokens over 700-3000 keys 185 us, of 16 rows
+// 260.)
 template <int DH>
 static yk_status launch_tca_rows(cudaStream_t st, bool pdl, int num_sms, const CUtensorMap& map, const Attn8Params& p,
                                  long long rows) {

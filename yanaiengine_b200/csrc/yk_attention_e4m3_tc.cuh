@@ -161,8 +161,9 @@ struct Turn {
     }
 };
 
-// The V warps and the queries' warp: a CTA's first queries, which everything waits for, are converted by all five.
-__device__ __forceinline__ void first_queries_bar() { asm volatile("bar.sync 1, 160;" ::: "memory"); }
+// The V warps and the queries' warp, where all five convert a span's queries: those of a CTA's first span, which
+// everything waits for, and with many rows every span's.
+__device__ __forceinline__ void queries_bar() { asm volatile("bar.sync 1, 160;" ::: "memory"); }
 __device__ __forceinline__ void v_bar() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 __device__ __forceinline__ float cap_score(const Attn8Params& p, float x) { return p.cap_log2 * tanh_cap(x * p.inv_cap_log2); }
 
