@@ -721,6 +721,91 @@ def test_attention_queries_with_an_element_far_above_the_rest(dtype, max_new, ti
 
 
 # ---------------------------------------------------------------------------
+# Calls among other work.
+# ---------------------------------------------------------------------------
+SHAPES = [("bf16", 1), ("bf16", 6), ("bf16", 1000), ("f32", 6)]
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_attention_keeps_its_place_in_the_stream(dtype, max_new):
+    """Launches overlap the end of the kernel before them: inputs written and results read by kernels right before and
+    after a call, round after round without waiting, are those of the round."""
+    a = Attention(28, 8, 2, 128, [(6, 700), (9, 90), (1, 400)], dtype)
+    g = torch.Generator().manual_seed(1)
+    qs = torch.randn(24, *a.q.shape, generator=g).to(a.q.dtype).to(dev())
+    want = []
+    for q in qs:
+        a.q.copy_(q)
+        a.call(max_new=max_new)
+        torch.cuda.synchronize()
+        want.append(a.out.clone())
+    outs = torch.zeros(24, *a.q.shape, dtype=a.q.dtype, device=dev())
+    torch.cuda.synchronize()
+    for i in range(24):
+        a.q.copy_(qs[i])
+        abi.attention_e4m3(a.q, a.out, a.pool, a.scales, a.layer, *a.d, a.ws, a.err, max_new=max_new)
+        outs[i].copy_(a.out)
+        a.out.zero_()
+    torch.cuda.synchronize()
+    assert torch.equal(outs, torch.stack(want)) and int(a.err) == 0
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_attention_twice_at_once(dtype, max_new):
+    """Two streams, a workspace each."""
+    calls = [Attention(29 + i, 8, 2, 128, [(6, 3000), (9, 90), (1, 400)], dtype) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for a in calls:
+        a.call(max_new=max_new)
+    torch.cuda.synchronize()
+    want = [a.out.clone() for a in calls]
+    outs = [torch.zeros(16, *a.out.shape, dtype=a.out.dtype, device=dev()) for a in calls]
+    torch.cuda.synchronize()
+    for i in range(16):
+        for a, st, out in zip(calls, streams, outs):
+            with torch.cuda.stream(st):
+                abi.attention_e4m3(a.q, out[i], a.pool, a.scales, a.layer, *a.d, a.ws, a.err, max_new=max_new)
+    torch.cuda.synchronize()
+    for a, w, out in zip(calls, want, outs):
+        assert all(torch.equal(w, o) for o in out) and int(a.err) == 0
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "bf16"])
+def test_append_keeps_its_place_in_the_stream(cache):
+    H, G, dh, T, n = 8, 2, 128, 40, 24
+    g = torch.Generator().manual_seed(2)
+    e4 = cache == "e4m3"
+    pool = torch.zeros(8, 1, 2, G, 16, dh, dtype=torch.uint8 if e4 else torch.bfloat16, device=dev())
+    scales = torch.full((8, 1, 2, G), 67, dtype=torch.uint8, device=dev()) if e4 else None
+    src = torch.randn(n, T, (H + 2 * G) * dh, generator=g).to(torch.bfloat16).to(dev())
+    qkv, q = torch.zeros_like(src[0]), torch.zeros(T, H, dh, dtype=torch.bfloat16, device=dev())
+    slots = torch.arange(T, dtype=torch.int32, device=dev()) + 5
+    err = torch.zeros(1, dtype=torch.int32, device=dev())
+    gain = torch.ones(dh, device=dev())
+
+    def rounds(wait):
+        got = torch.zeros(n, T, H, dh, dtype=torch.bfloat16, device=dev())
+        cells = torch.zeros(n, *pool.shape, dtype=pool.dtype, device=dev())
+        pool.zero_()
+        if e4:
+            scales.fill_(67)
+        torch.cuda.synchronize()
+        for i in range(n):
+            qkv.copy_(src[i])
+            abi.kv_append(pool, scales, 0, qkv, q, slots, None, gain, gain, 1e-6, err, H)
+            got[i].copy_(q)
+            cells[i].copy_(pool)
+            qkv.zero_()
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return got, cells
+
+    one, other = rounds(True), rounds(False)
+    assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1]) and int(err) == 0
+
+
+# ---------------------------------------------------------------------------
 # Both, as a decoding step uses them.
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

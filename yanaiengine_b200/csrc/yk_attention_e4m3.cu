@@ -276,8 +276,10 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
 
             // ---- queries to B fragments in shared memory, 8 rows at a time: column n = lane / 4,
             // dims 64 h + 16 c + 4 s + {0, 1 | 2, 3} of k-step 4 h + s
+            // (rows that the span does not fill are zeros: what lay there before must not decide when a warp moves its
+            // references, which shows in the last bit)
 #pragma unroll 1
-            for (int u = warp; u * 8 < rows; u += 4) {
+            for (int u = warp; u * 8 < R; u += 4) {
                 const int row = u * 8 + r;
                 load_q(sg, u);
                 float amax = 0.f;
@@ -718,10 +720,10 @@ yk_status attention_e4m3_check(const yk_attention_e4m3_args& a) {
     const int64_t es = a.dtype == YK_DTYPE_F32 ? 4 : 2, row = (int64_t)a.n_heads * a.pages.head_dim;
     YK_ARG(a.q_stride >= row && a.q_stride * es % 16 == 0 && a.out_stride >= row && a.out_stride * es % 16 == 0,
            "q_stride / out_stride must cover a row and be multiples of 16 bytes");
-    // (tiles have 8 rows at least, and their pages are counted in 31 bits)
+    // (tiles have 8 rows at least, and their pages and costs are counted in 32 bits)
     const int64_t tiles = (int64_t)a.T * (a.n_heads / a.pages.n_kv_heads) / 8 + a.B, heads = a.pages.n_kv_heads;
-    if ((int64_t)a.T * a.n_heads >= (int64_t)1 << 31 || (double)tiles * (double)heads * a.max_blocks >= 2147483648.0) {
-        yk_set_error("unsupported: T * n_heads or (T * n_heads / 8 + B * n_kv_heads) * max_blocks is 2^31 or more; "
+    if ((int64_t)a.T * a.n_heads >= (int64_t)1 << 31 || (double)tiles * (double)heads * (a.max_blocks + (double)A8_COST) >= 2147483648.0) {
+        yk_set_error("unsupported: T * n_heads or (T * n_heads / 8 + B * n_kv_heads) * (max_blocks + 8) is 2^31 or more; "
                      "split the batch");
         return YK_ERR_UNSUPPORTED;
     }
