@@ -226,7 +226,9 @@ yk_status yk_kv_pool_create_layers(yk_engine* e, const yk_model_config* cfg, int
  * (a quarter) of the memory of yk_kv_pool_create's, and of the bytes attention
  * reads.  Every forward call takes it in the other's place (split pools: both of
  * them); the keys and values of a step are stored by yk_kv_append's kernel and
- * read by yk_attention_e4m3's.  Not for ref_compat models. */
+ * read by yk_attention_e4m3's.  A block belongs to one sequence of a step: two
+ * that write to the same one leave its scale and cells undefined.  Not for
+ * ref_compat models. */
 yk_status yk_kv_pool_create_e4m3(yk_engine* e, const yk_model_config* cfg, int32_t num_blocks, int32_t layers,
                                  yk_kv_pool** out);
 void      yk_kv_pool_destroy(yk_kv_pool* p);
@@ -370,7 +372,7 @@ yk_status yk_kv_append(int32_t device, void* stream, const yk_kv_append_args* ar
  * are held to 2^-21 of their row's largest value (F32: to 22 bits).
  * At most 1024 query heads to a KV head and 2^25 columns of block_tables;
  * YK_ERR_UNSUPPORTED from T * n_heads or (T * n_heads / 8 + B * n_kv_heads) *
- * max_blocks = 2^31 on: split the batch. */
+ * (max_blocks + 8) = 2^31 on: split the batch. */
 typedef struct yk_attention_e4m3_args {
     yk_kv_pages    pages;
     int32_t        layer;

@@ -410,7 +410,6 @@ extern "C" void yk_model_destroy(yk_model* m) {
     if (m->gemm_stamps) cudaFree(m->gemm_stamps);
     if (m->chain_bar) cudaFree(m->chain_bar);
     if (m->gemm_counters) cudaFree(m->gemm_counters);
-    if (m->attn8_ws) cudaFree(m->attn8_ws);
     delete m;
 }
 
@@ -562,6 +561,8 @@ static yk_status create_pool(yk_engine* e, const yk_model_config* cfg, int32_t n
         const size_t n = (size_t)num_blocks * n_pool_layers * 2 * cfg->n_kv_heads;
         err = cudaMalloc(&p->scales, n);
         if (err == cudaSuccess) err = cudaMemset(p->scales, yk::KV8_BIAS + yk::KV8_EMIN, n);
+        // (the first step, on the engine's own stream, must not be overtaken by these)
+        if (err == cudaSuccess) err = cudaStreamSynchronize(nullptr);
         if (err != cudaSuccess) {
             if (p->scales) cudaFree(p->scales);
             cudaFree(p->data);
@@ -809,8 +810,10 @@ static yk_status forward_impl(yk_model* m, yk_kv_pool* pool, const uint32_t* tok
         YK_TRY(dalloc(m, (void**)&m->qkv_raw, (size_t)c.max_tokens * (c.n_heads + 2 * c.n_kv_heads) * c.head_dim * 4));
     if (e4 && !m->attn8_ws) {
         const size_t n = yk::attention_e4m3_ws_bytes(e->num_sms, c.head_dim);
-        YK_CHECK_CUDA(cudaMalloc(&m->attn8_ws, n));
-        YK_CHECK_CUDA(cudaMemsetAsync(m->attn8_ws, 0, n, e->stream));  // (its first user is on the same stream)
+        uint8_t* ws = nullptr;
+        YK_TRY(dalloc(m, (void**)&ws, n));
+        YK_CHECK_CUDA(cudaMemsetAsync(ws, 0, n, e->stream));  // (its first user is on the same stream)
+        m->attn8_ws = ws;
         m->attn8_ws_bytes = n;
     }
     if (c.dtype == YK_DTYPE_BF16 && !e4) {
