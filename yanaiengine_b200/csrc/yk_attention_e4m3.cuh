@@ -55,7 +55,7 @@ __device__ __forceinline__ float tanh_cap(float z) {
     return fabsf(z) < 0.25f ? t : e;
 }
 
-// x / (H / G), x below 64 + H / G (exact: x * (H / G) < 2^32).
+// x / (H / G), x below 128 + H / G (exact: x * (H / G) < 2^32).
 __device__ __forceinline__ int div_rep(const Attn8Params& p, int x) {
     return p.rep_magic ? (int)__umulhi((unsigned)x, p.rep_magic) : x;
 }

@@ -7,7 +7,7 @@
 //   producers  one warp for K, one for V (a warp issues a copy in about 85 cycles,
 //              whatever its size): table entries and scale bytes; K pages by TMA
 //              (128- or 64-byte swizzle), V pages by bulk copy, into rings of tiles
-//   queries    the next span's queries into e4m3 pairs
+//   queries    the next span's queries into pairs of 8-bit terms
 //   MMA        S^T[128 keys x 2R] = K Q^T (kind::f8f6f4), O^T[dims x R] += V^T P^T
 //              (kind::f16), accumulators in TMEM, S^T and O^T double-buffered
 //   softmax    two groups of 4 warps, half of the rows each, one key a thread: scores
@@ -19,7 +19,8 @@
 // row's largest value at least).  For few rows both are e4m3, the second scaled by
 // 16, as separate columns of one product; from 24 rows on the second is e5m2 (the
 // remainder is at most 8 units of the last bit, 3 bits wide) and its product adds
-// to the first's: half the scores to read back (prompt 835 -> 813 us).  V converts once for all rows of the tile (R up to 64).
+// to the first's: half the scores to read back (64 rows: 835 -> 813 us).  V
+// converts once for all rows of the tile (R up to 48).
 //
 // Weights as in the other kernel: p = 2^(x + e_V - m), f16.  The reference m of a
 // row is kept by its group, lazily: it is set 2^3 below a row's first weights
