@@ -247,12 +247,14 @@ __device__ __forceinline__ void append_block(const AppendParams& p, int t, int s
 // Bytes bound it: every row is read once.  What the shape is after is loads in
 // flight and few instructions a byte: 16 bytes of bf16 a lane, STEPS rows of
 // loads a warp where there are rows enough, one where there are not (decode).
-// Measured, 32 query and 8 KV heads of 128: 8,197 tokens of bf16 into e4m3 cells 56
-// us (162 MB, 2.9 TB/s, 44 % of a copy's rate: a third of the warps fit, 72
-// registers, and wait for loads); 2,048 tokens into bf16 cells 10.7 us (68 MB, 97 %
-// with what stays in L2); 192 tokens 5.7 us and one token 2.8 us, the launch.
+// Measured, 32 query and 8 KV heads of 128: 8,197 tokens of bf16 into e4m3 cells 52
+// us (162 MB, 3.1 TB/s, 47 % of a copy's rate: a third of the warps fit beside 8 KB
+// of staging each, and wait for loads; bound to 72 registers for a seventh CTA that
+// the staging does not leave room for, 56 us); 2,048 tokens into bf16 cells 10.6 us
+// (68 MB, 97 % with what stays in L2); 192 tokens 5.6 us and one token 2.7 us, the
+// launch.
 template <typename SRC, typename DST, bool E4M3, int DH, int STEPS>
-__global__ void __launch_bounds__(128, DH == 256 ? 3 : 7) kv_append_kernel(const __grid_constant__ AppendParams p, unsigned row_blocks, int tile) {
+__global__ void __launch_bounds__(128, DH == 256 ? 3 : 6) kv_append_kernel(const __grid_constant__ AppendParams p, unsigned row_blocks, int tile) {
     extern __shared__ __align__(16) float append_stage[];
     pdl_trigger();
     pdl_wait();
