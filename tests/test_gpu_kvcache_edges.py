@@ -1,0 +1,63 @@
+"""Attention over an e4m3 paged cache at the ends of its arguments' ranges: cells and queries that are not
+finite under a soft cap, positions far below zero, queries, caps and windows as large as their types hold.
+The tolerances are kvcache_ref.attention_bound's throughout."""
+import math
+
+import pytest
+import torch
+
+import kvcache_ref as ref
+from test_gpu_kvcache import Attention
+
+pytestmark = pytest.mark.gpu
+
+# every kernel: bf16 tiles of 8, of 24 and of 128 rows (32 at head_dim 256), fp32 tiles of 8 and of 32 (16)
+SHAPES = [("bf16", 1), ("bf16", 6), ("bf16", 1000), ("f32", 1), ("f32", 6)]
+
+
+def reference(a, **kw):
+    return ref.attention(a.q, a.pool, a.scales, a.layer, a.starts, a.ctx, a.tables, **kw)
+
+
+def assert_rows(a, want, poisoned):
+    """Elements of `poisoned` are NaN, the others right."""
+    got = a.out.double().cpu()
+    assert torch.isnan(got[poisoned]).all()
+    bound = ref.attention_bound(*want, got.shape[-1], a.out.dtype)
+    assert ((got - want[0]).abs()[~poisoned] <= bound[~poisoned]).all()
+    assert int(a.err) == 0
+
+
+# ---------------------------------------------------------------------------
+# NaN.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("which", [0, 1])
+def test_nan_cell_reaches_those_who_see_it(dtype, max_new, dh, cap, which):
+    """A NaN in the K or V of a new token's cell: earlier tokens are untouched, later ones NaN, with a soft cap too."""
+    a = Attention(16, 4, 2, dh, [(8, 60), (1, 20), (9, 300)], dtype)
+    want = reference(a, cap=cap)
+    j = 60 - 3  # the sixth new token's cell
+    a.pool[a.tables[0, j // 16], 1, which, 0, j % 16, 37] = 0xFF
+    a.call(max_new=max_new, cap=cap)
+    torch.cuda.synchronize()
+    poisoned = torch.zeros(a.out.shape, dtype=torch.bool)
+    poisoned[5:8, :2, slice(None) if which == 0 else 37] = True  # heads 0, 1 read KV head 0
+    assert_rows(a, want, poisoned)
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("cap,window", [(0.0, 0), (30.0, 0), (30.0, 40)])
+def test_nan_query_reaches_its_row_only(dtype, max_new, dh, cap, window):
+    a = Attention(17, 4, 2, dh, [(8, 60), (1, 20), (9, 300)], dtype)
+    want = reference(a, cap=cap, window=window)
+    poisoned = torch.zeros(a.out.shape, dtype=torch.bool)
+    for t, h, d in ((0, 0, 0), (5, 3, 63), (8, 1, 17), (13, 2, 40)):
+        a.q[t, h, d] = math.nan
+        poisoned[t, h] = True
+    a.call(max_new=max_new, cap=cap, window=window)
+    torch.cuda.synchronize()
+    assert_rows(a, want, poisoned)

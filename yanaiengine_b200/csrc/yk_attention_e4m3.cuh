@@ -47,10 +47,15 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float fmin_nan(float a, float b) {  // (fminf passes over a NaN)
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 // tanh to a few 2^-24 of its value: 1 - 2 / (1 + e^2z) away from 0, the odd
-// series z - z^3/3 + 2z^5/15 - 17z^7/315 near it.
+// series z - z^3/3 + 2z^5/15 - 17z^7/315 near it.  NaN stays NaN.
 __device__ __forceinline__ float tanh_cap(float z) {
-    const float e = 1.f - __fdividef(2.f, 1.f + ex2(fminf(z * 2.8853900817779268f, 126.f)));
+    const float e = 1.f - __fdividef(2.f, 1.f + ex2(fmin_nan(z * 2.8853900817779268f, 126.f)));
     const float q = z * z, t = fmaf(fmaf(fmaf(-17.f / 315.f, q, 2.f / 15.f), q, -1.f / 3.f), q, 1.f) * z;
     return fabsf(z) < 0.25f ? t : e;
 }
