@@ -61,3 +61,17 @@ def test_nan_query_reaches_its_row_only(dtype, max_new, dh, cap, window):
     a.call(max_new=max_new, cap=cap, window=window)
     torch.cuda.synchronize()
     assert_rows(a, want, poisoned)
+
+
+# ---------------------------------------------------------------------------
+# Positions below zero.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_positions_far_below_zero_give_zeros(dtype, max_new):
+    """Whole query tiles without a key, hundreds of positions below zero, after calls that left cells of others in
+    shared memory."""
+    a = Attention(31, 4, 2, 64, [(40, 3000), (400, 400)], dtype)
+    a.check(max_new=max_new)
+    a.ctx[1] = 2  # 400 new tokens, two positions
+    a.check(max_new=max_new)
+    assert (a.out[40:438] == 0).all()

@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
             const int k_end = (sg.v + sg.n - v0 - part + nparts - 1) >> (2 - p.lg);
             int j0 = 0, ek = 0, ev = 0;
             uint32_t page = my_ring;
-            // page i has arrived: its place, first key and exponents (a page that is not there keeps its
-            // cells masked, whatever its slot holds)
+            // page i has arrived: its place, first key (-1: a page that is not there, no row sees its cells,
+            // whatever its slot holds) and exponents
             const auto take = [&](int i) {
                 if (i >= base + 32) {
                     base += 32;
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
                 ek = kv8_exponent(__shfl_sync(0xffffffffu, kb, i & 31));
                 ev = kv8_exponent(__shfl_sync(0xffffffffu, vb, i & 31));
                 page = my_ring + (uint32_t)(out_slot * C::PAGE);
-                j0 = id >= 0 ? (sg.page + (v0 + part + nparts * i - sg.v)) * 16 : 0x7fffff00;
+                j0 = id >= 0 ? (sg.page + (v0 + part + nparts * i - sg.v)) * 16 : -1;
                 if (!dead && !mbar_wait_bounded(full + out_slot * 8, (uint32_t)out_phase)) {
                     if (lane == 0) raise_err(p.err, YK_DEV_ERR_TIMEOUT);
                     dead = true;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
             while (k < k_end) {
                 const uint32_t held = page;
                 const int held_j0 = j0, slot = (out_slot == 0 ? depth : out_slot) - 1;
-                const bool plain = p.cap <= 0.f && j0 + 15 <= sg.pos && (p.window <= 0 || pos_last - j0 < p.window);
+                const bool plain = p.cap <= 0.f && j0 >= 0 && j0 + 15 <= sg.pos && (p.window <= 0 || pos_last - j0 < p.window);
                 uint32_t pb[TERMS][NT][2];
                 if (active) {
                     // scores -> x + e_V in the log2 domain; row 2c: s[0], s[2], row 2c + 1: s[1], s[3]
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
                             for (int j = 0; j < 2; ++j) {
                                 const int row = my0 + nt * 8 + 2 * c + j;
                                 const unsigned back = (unsigned)(sg.pos + row_token(row) - sigma - j0);  // query minus key
-                                const unsigned w = row < rows ? (p.window > 0 ? (unsigned)p.window : 0x80000000u) : 0u;
+                                const unsigned w = row < rows && j0 >= 0 ? (p.window > 0 ? (unsigned)p.window : 0x80000000u) : 0u;
                                 s[nt][j] = back < w ? s[nt][j] + shift : -INFINITY;
                                 s[nt][j + 2] = back - 8 < w ? s[nt][j + 2] + shift : -INFINITY;
                             }
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
                                     const int dim = bx * 128 + v_dim + byte;
                                     for (int row = my0; row < min(rows, my0 + C::ROWS); ++row) {
                                         const int back = sg.pos + row_token(row) - held_j0 - key;
-                                        if (back >= 0 && (p.window <= 0 || back < p.window)) {
+                                        if (held_j0 >= 0 && back >= 0 && (p.window <= 0 || back < p.window)) {
                                             atomicOr(&s_nan[row * (DH / 32) + (dim >> 5)], 1u << (dim & 31));
                                             s_flag[0] = 1;
                                         }
