@@ -75,3 +75,35 @@ def test_positions_far_below_zero_give_zeros(dtype, max_new):
     a.ctx[1] = 2  # 400 new tokens, two positions
     a.check(max_new=max_new)
     assert (a.out[40:438] == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# Queries at the end of their type's range.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("mag", [6e37, 1e36, 1e33, 1e-33, 1e-35])
+def test_queries_of_any_magnitude(dtype, max_new, dh, mag):
+    a = Attention(24, 4, 2, dh, [(3, 200), (9, 40)], dtype)
+    a.q = (a.q.double() * mag).to(a.q.dtype)
+    assert torch.isfinite(a.q).all()
+    a.check(scale=float(dh ** -0.5 / mag), max_new=max_new)
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_infinite_query_reaches_its_row_only(dtype, max_new, dh, cap):
+    """All its scores are infinite or NaN: so is no softmax of them.  A token without a key still gets zeros."""
+    a = Attention(18, 4, 2, dh, [(8, 60), (1, 20), (9, 300), (5, 40)], dtype)
+    a.ctx[3] = 2
+    want = reference(a, cap=cap)
+    poisoned = torch.zeros(a.out.shape, dtype=torch.bool)
+    for t, h, d, x in ((0, 0, 0, math.inf), (5, 3, 63, -math.inf), (8, 1, 17, math.inf), (13, 2, 40, -math.inf)):
+        a.q[t, h, d] = x
+        poisoned[t, h] = True
+    a.q[18, 1, 5] = math.inf
+    a.call(max_new=max_new, cap=cap)
+    torch.cuda.synchronize()
+    assert_rows(a, want, poisoned)
+    assert (a.out[18:21] == 0).all()

@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
                                  fmaxf(fabsf(__uint_as_float(qw[h].z)), fabsf(__uint_as_float(qw[h].w))));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                // shift by 2^up: amax = m * 2^E, 1 <= m < 2, to m * 2^14
-                const int up = amax == 0.f ? 0 : max(-100, min(100, 14 + 127 - (int)(__float_as_uint(amax) >> 23)));
+                // shift by 2^up: amax = m * 2^E, 1 <= m < 2, to m * 2^14 (an infinite element: its second term is NaN,
+                // and so are the row's scores)
+                const int up = amax == 0.f ? 0 : min(126, 14 + 127 - (int)(__float_as_uint(amax) >> 23));  // -114 at least
                 const float f = exp2_int(up);
                 if (c == 0) s_rf[row] = p.scale_log2 * exp2_int(-up);
                 const uint32_t dst = smem_u32(shared + C::QOFF) + (uint32_t)(u * TERMS * KS * 256 + lane * 16);

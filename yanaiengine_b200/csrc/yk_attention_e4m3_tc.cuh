@@ -348,10 +348,11 @@ __device__ __forceinline__ void convert_queries(const Attn8Params& p, const Seg&
         }
 #pragma unroll
         for (int o = 1; o < LPR; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // 2^-e brings the row's largest value to at most 448
+        // 2^-e brings the row's largest value to at most 448.  An infinite one has no place in the terms, which
+        // saturate: its row's become NaN, as the softmax of its scores is
         const uint32_t bits = __float_as_uint(amax);
-        const int e = amax == 0.f ? 0 : max(-100, min(100, (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0)));
-        const float g = exp2_int(-e);
+        const int e = amax == 0.f ? 0 : max(-126, (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0));  // 120 at most
+        const float g = bits == 0x7f800000u ? __int_as_float(0x7fffffff) : exp2_int(-e);
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int z = 0; z < 4; ++z) {
@@ -367,7 +368,7 @@ __device__ __forceinline__ void convert_queries(const Attn8Params& p, const Seg&
             }
         }
         if (row < R && live) {
-            if (c16 == 0) s_rf[row] = p.scale_log2 * exp2_int(e);
+            if (c16 == 0) s_rf[row] = fminf(p.scale_log2 * exp2_int(e), A8_LARGEST);  // (finite: a score of 0 stays 0)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int n = row + t * R;
