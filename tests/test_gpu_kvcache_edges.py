@@ -107,3 +107,15 @@ def test_infinite_query_reaches_its_row_only(dtype, max_new, dh, cap):
     torch.cuda.synchronize()
     assert_rows(a, want, poisoned)
     assert (a.out[18:21] == 0).all()
+
+
+# ---------------------------------------------------------------------------
+# Windows and caps at the end of their type's range.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 30])
+def test_window_as_large_as_it_gets_masks_nothing(dtype, max_new, window):
+    """... in a tile that begins below position zero too."""
+    a = Attention(32, 8, 2, 128, [(40, 60), (9, 300)], dtype)
+    a.ctx[0] = 17
+    a.check(max_new=max_new, window=window)

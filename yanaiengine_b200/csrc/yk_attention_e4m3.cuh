@@ -86,7 +86,7 @@ __device__ __forceinline__ Span span_of(const Attn8Params& p, int n, int ctx, in
     const int first = ctx - n + s.tok;
     const int last = first + div_rep(p, s.rem + s.rows - 1);
     s.pend = (min(max(last, -1), p.max_blocks * 16 - 1) + 16) >> 4;
-    s.page = p.window > 0 ? min(max(0, first - p.window + 1) >> 4, s.pend) : 0;
+    s.page = p.window > 0 ? min(max(0, max(first, 0) - p.window + 1) >> 4, s.pend) : 0;
     return s;
 }
 
