@@ -119,3 +119,10 @@ def test_window_as_large_as_it_gets_masks_nothing(dtype, max_new, window):
     a = Attention(32, 8, 2, 128, [(40, 60), (9, 300)], dtype)
     a.ctx[0] = 17
     a.check(max_new=max_new, window=window)
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("cap", [3.4028234e38, 1e38, 1e36, 1e-36, 1e-39])
+def test_caps_of_any_size(dtype, max_new, cap):
+    """A huge one changes nothing, a tiny one makes all weights equal."""
+    Attention(33, 8, 2, 128, [(6, 300), (9, 40)], dtype).check(max_new=max_new, cap=cap)

@@ -792,9 +792,11 @@ yk_status attention_e4m3_launch(cudaStream_t st, bool pdl, int num_sms, const yk
     p.window = a.window;
     const float scale = a.scale > 0.f ? a.scale : 1.0f / std::sqrt((float)a.pages.head_dim), log2e = 1.4426950408889634f;
     p.scale_log2 = scale * log2e;
-    p.cap = a.cap;
-    p.cap_log2 = a.cap * log2e;
-    p.inv_cap_log2 = a.cap > 0.f ? 1.0f / p.cap_log2 : 0.f;
+    // (a cap of 2^125 changes no score that fp32 holds apart, one of 2^-125 makes all weights equal: beyond them
+    // cap * log2(e) or its inverse has no place in fp32)
+    p.cap = a.cap > 0.f ? std::min(std::max(a.cap, 0x1p-125f), 0x1p125f) : 0.f;
+    p.cap_log2 = p.cap * log2e;
+    p.inv_cap_log2 = p.cap > 0.f ? 1.0f / p.cap_log2 : 0.f;
     uint8_t* const ws = reinterpret_cast<uint8_t*>(a.workspace);
     const unsigned rep = (unsigned)(a.n_heads / a.pages.n_kv_heads);
     p.rep_magic = rep == 1 ? 0u : (unsigned)((0x100000000ull + rep - 1) / rep);
