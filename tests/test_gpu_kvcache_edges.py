@@ -77,6 +77,17 @@ def test_positions_far_below_zero_give_zeros(dtype, max_new):
     assert (a.out[40:438] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_contexts_below_zero_give_zeros(dtype, max_new):
+    """Every position of such a sequence is below zero, down to the lowest length there is."""
+    a = Attention(34, 4, 2, 64, [(7, 300), (40, 40), (1, 30), (9, 90)], dtype)
+    a.check(max_new=max_new)
+    for low in (-1, -2 ** 30, -2 ** 31 + 39, -2 ** 31):
+        a.ctx[1] = a.ctx[2] = low
+        a.check(max_new=max_new)
+        assert (a.out[7:48] == 0).all()
+
+
 # ---------------------------------------------------------------------------
 # Queries at the end of their type's range.
 # ---------------------------------------------------------------------------

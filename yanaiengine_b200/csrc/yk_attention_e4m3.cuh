@@ -96,6 +96,8 @@ __device__ __forceinline__ int new_tokens(const Attn8Params& p, int b, int& star
     const int end = p.q_starts[b + 1];
     return start >= 0 && end >= start && end <= p.T && (b > 0 || start == 0) ? end - start : -1;
 }
+// Its length.  (Below 0 all positions are, as they are at 0; ctx - n stays inside 32 bits.)
+__device__ __forceinline__ int context_of(const Attn8Params& p, int b) { return max(p.ctx[b], 0); }
 
 
 // A thread's sequences and this CTA's range of units (LEAST at least), [lo, hi) of the spans laid end to end.  A span has COST units
@@ -127,7 +129,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     int spans = 0;
     for (int b = w.b_lo; b < w.b_hi; ++b) {
         int start;
-        const int n = new_tokens(p, b, start), ctx = p.ctx[b];
+        const int n = new_tokens(p, b, start), ctx = context_of(p, b);
         if (b == w.b_lo) {
             w.start = start;
             w.n = n;
@@ -175,7 +177,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
             int start = w.start, n = w.n, ctx = w.ctx;
             if (b > w.b_lo) {
                 n = new_tokens(p, b, start);
-                ctx = p.ctx[b];
+                ctx = context_of(p, b);
             }
             const int q_hi = b == w.b_lo ? w.q_hi : tiles_of(n, R, rep);
             for (int qt = b == w.b_lo ? w.q_lo : 0; qt < q_hi; ++qt) {
@@ -213,7 +215,7 @@ __device__ __forceinline__ void a8_list(const Attn8Params& p, int R, int rep, co
         for (int b = b_lo; b < b_hi; ++b) {
             if (b > b_lo) {
                 n = new_tokens(p, b, start);
-                ctx = p.ctx[b];
+                ctx = context_of(p, b);
                 q_lo = 0;
                 q_hi = tiles_of(n, R, rep);
             }
