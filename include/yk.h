@@ -390,7 +390,9 @@ typedef struct yk_attention_e4m3_args {
     int64_t        q_stride;
     void*          out;
     int64_t        out_stride;
-    const int32_t* q_starts;     /* [B + 1], from 0, not falling, at most T          */
+    const int32_t* q_starts;     /* [B + 1], from 0, not falling, at most T (a sequence
+                                    that does not fit is left out; nothing is done if
+                                    the others bring more than T tokens together)    */
     const int32_t* context_lens; /* [B]                                             */
     const int32_t* block_tables; /* [B][max_blocks]                                 */
     void*          workspace;

@@ -137,3 +137,38 @@ def test_window_as_large_as_it_gets_masks_nothing(dtype, max_new, window):
 def test_caps_of_any_size(dtype, max_new, cap):
     """A huge one changes nothing, a tiny one makes all weights equal."""
     Attention(33, 8, 2, 128, [(6, 300), (9, 40)], dtype).check(max_new=max_new, cap=cap)
+
+
+# ---------------------------------------------------------------------------
+# q_starts that fall.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_sequences_that_overlap_are_not_begun(dtype, max_new):
+    """Starts that fall and rise again give 128 sequences the same 8192 rows, more work than 32 bits count (8 heads x
+    8192 tokens x 131,072 keys each): nothing is written, the error word says so, and the next call is right."""
+    a = Attention(35, 8, 8, 64, [(6, 300), (9, 40)], dtype)
+    right = a.q, a.out, a.starts, a.ctx, a.tables
+    T, B = 8192, 256
+    a.q = torch.zeros(T, 8, 64, dtype=a.q.dtype, device=a.q.device)
+    a.out = torch.full_like(a.q, 7.0)
+    a.starts, a.ctx = [T * (b % 2) for b in range(B + 1)], [131072] * B
+    a.tables = torch.zeros(B, 8192, dtype=torch.int32)
+    a.call(max_new=max_new)
+    torch.cuda.synchronize()
+    assert (a.out == 7.0).all() and int(a.err) == 1
+    a.err.zero_()
+    a.q, a.out, a.starts, a.ctx, a.tables = right
+    a.check(max_new=max_new)
+
+
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+def test_a_sequence_whose_starts_do_not_fit_leaves_the_others_right(dtype, max_new):
+    a = Attention(36, 8, 2, 64, [(2, 30), (3, 40), (4, 50)], dtype)
+    want = reference(a)
+    a.starts = [0, 2, 5, 900]  # the last one ends past T
+    a.call(max_new=max_new)
+    torch.cuda.synchronize()
+    got = a.out.double().cpu()
+    bound = ref.attention_bound(*want, 64, a.out.dtype)
+    assert ((got - want[0]).abs()[:5] <= bound[:5]).all()
+    assert (got[5:] == 7.0).all() and int(a.err) == 1

@@ -127,6 +127,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     w.units = 0;  // (the host sees to it that all pages together stay below 2^31)
     w.start = w.n = w.ctx = w.q_lo = w.q_hi = 0;
     int spans = 0;
+    bool misfit = false;
     for (int b = w.b_lo; b < w.b_hi; ++b) {
         int start;
         const int n = new_tokens(p, b, start), ctx = context_of(p, b);
@@ -138,6 +139,7 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
             w.q_lo = min(tiles, ((int)threadIdx.x & ((1 << share) - 1)) * each);
             w.q_hi = min(tiles, w.q_lo + each);
         }
+        misfit |= n < 0;
         if (n < 0 || (n > 0 && ctx > p.max_blocks * 16LL)) raise_err(p.err, YK_DEV_ERR_BOUNDS);
         const int q_hi = b == w.b_lo ? w.q_hi : tiles_of(n, R, rep);
         for (int qt = b == w.b_lo ? w.q_lo : 0; qt < q_hi; ++qt) {
@@ -160,11 +162,28 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
         s_scan[warp] = w.at0;
         s_scan[WARPS + warp] = (unsigned)w.ord0;
     }
-    __syncthreads();
+    misfit = __syncthreads_or(misfit);
     const unsigned wu = lane < WARPS ? s_scan[lane] : 0u, ws = lane < WARPS ? s_scan[WARPS + lane] : 0u;
     const unsigned total = __reduce_add_sync(0xffffffffu, wu);
     w.at0 += __reduce_add_sync(0xffffffffu, lane < warp ? wu : 0u) - w.units;
     w.ord0 += (int)__reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u) - spans;
+    if (misfit) {
+        // starts that fall may give the same rows to many sequences, and these more units than 32 bits hold: nothing
+        // is begun where they bring more than T tokens together (1e-3 is more than fp32 rounds 2100 terms)
+        float tokens = 0.f;
+        for (int b = w.b_lo; b < w.b_hi; ++b) {
+            int start;
+            if (threadIdx.x % (1u << share) == 0) tokens += (float)max(new_tokens(p, b, start), 0);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+        __syncthreads();
+        if (lane == 0) s_scan[warp] = __float_as_uint(tokens);
+        __syncthreads();
+        tokens = 0.f;
+        for (int i = 0; i < WARPS; ++i) tokens += __uint_as_float(s_scan[i]);
+        if (tokens > (float)p.T * 1.001f) return false;
+    }
     w.per = max((unsigned)LEAST, (total + gridDim.x - 1) / gridDim.x);
     w.lo = min(total, blockIdx.x * w.per);
     w.hi = min(total, w.lo + w.per);
