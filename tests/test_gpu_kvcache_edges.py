@@ -1,13 +1,15 @@
-"""Attention over an e4m3 paged cache at the ends of its arguments' ranges: cells and queries that are not
-finite under a soft cap, positions far below zero, queries, caps and windows as large as their types hold.
-The tolerances are kvcache_ref.attention_bound's throughout."""
+"""The operators on an e4m3 paged cache at the ends of their arguments' ranges: cells and queries that are not
+finite under a soft cap, positions far below zero, queries, caps and windows as large as their types hold, starts
+that fall, steps that are padding for the most part.
+The tolerances are kvcache_ref.attention_bound's and Append.compare's throughout."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 import kvcache_ref as ref
-from test_gpu_kvcache import Attention
+from test_gpu_kvcache import Append, Attention
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +174,28 @@ def test_a_sequence_whose_starts_do_not_fit_leaves_the_others_right(dtype, max_n
     bound = ref.attention_bound(*want, 64, a.out.dtype)
     assert ((got - want[0]).abs()[:5] <= bound[:5]).all()
     assert (got[5:] == 7.0).all() and int(a.err) == 1
+
+
+# ---------------------------------------------------------------------------
+# Append: long runs of padding.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("cache", ["e4m3", "bf16"])
+@pytest.mark.parametrize("gap", [1, 31, 32, 33, 255, 256, 287, 288, 289, 320, 700])
+def test_append_rows_far_apart(cache, gap):
+    """Padding between the rows of a block, between blocks, before the first row and behind the last one."""
+    a = Append(37, 4, 2, 64, [(21, 40), (1, 16), (16, 32), (2, 5)], cache=cache)
+    n, lead = len(a.slots), 40
+    at = lead + np.arange(n) + gap * ((np.arange(n) + 1) // 2)  # a gap before every other row
+    T = int(at[-1]) + 1 + 2 * gap
+    at_d = torch.as_tensor(at).to(a.qkv.device)
+
+    def spread(x, fill):
+        y = torch.full((T, *x.shape[1:]), fill, dtype=x.dtype, device=x.device)
+        y[at_d] = x
+        return y
+
+    a.qkv, a.q, a.rope = spread(a.qkv, 3.0), spread(a.q, 7.0), spread(a.rope, 1.0)
+    slots = np.full(T, -1, np.int32)
+    slots[at] = a.slots
+    a.slots = slots
+    a.check()
