@@ -318,7 +318,8 @@ yk_status yk_kv_pool_pages(yk_kv_pool* p, yk_kv_pages* out);
  *             (cos, sin), fp32 (S/gemm.metal:674-682); null: none
  *   store     queries to q_out, keys and values to cache slot slots[t] =
  *             block * 16 + offset of layer `layer`.
- * A negative slot marks a row of padding: nothing of it is read or written.  No
+ * A negative slot marks a row of padding: nothing of it is written, and its values
+ * reach nothing (its place in qkv and rope is there, and may be read).  No
  * slot may appear twice, and the rows of one block must follow one another (rows
  * of padding may lie between them).
  * YK_KV_E4M3: the exponent of a block's K (or V) of one head is the smallest in
