@@ -305,7 +305,12 @@ template <typename SRC, typename DST, bool E4M3, int DH>
 static cudaError_t launch_append_dh(cudaStream_t st, bool pdl, int sms, const AppendParams& p) {
     constexpr int RPW = 256 / DH, STEPS = 4;
     const int heads = E4M3 ? p.H : p.H + 2 * p.G;
-    const long long warps = (long long)sms * 28;
+    // Several rows a warp, and several rows to look through, once that leaves this many warps an SM.  16-bit and fp32
+    // pools: 24, as many as run at once (384 tokens, 32 + 16 heads of 128 into bf16 cells: 4.1 us, 4.9 with 12).
+    // e4m3 pools, whose block warps take half of the room: 12 (768 tokens 10.4 us, 12.1 with 24; 1,536 tokens 14.4
+    // and 14.7; heads of 256 15.8 and 20.8, 21.1 and 23.7; heads of 64 7.4 and 7.9, 8.5 and 10.4).  Up to 192 tokens
+    // and from 8,192 on the two are the same.
+    const long long warps = (long long)sms * (E4M3 ? 12 : 24);
     const auto tasks = [&](int steps) { return (long long)p.T * ((heads + steps * RPW - 1) / (steps * RPW)); };
     const int steps = tasks(STEPS) >= warps ? STEPS : 1;  // (several rows a warp once that still fills the device)
     const unsigned row_blocks = (unsigned)((tasks(steps) + 3) / 4);
