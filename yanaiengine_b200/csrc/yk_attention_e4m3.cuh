@@ -112,6 +112,19 @@ struct A8Work {
     int first, nspans;    // spans of the range
 };
 
+// A warp, where some q_starts do not fit: whether the sequences that do bring more than T tokens together.  (Starts that
+// fall may give the same rows to many, and these more units than 32 bits hold.)
+__device__ __forceinline__ bool a8_overlap(const Attn8Params& p) {
+    unsigned tokens = 0;
+    for (int b = threadIdx.x & 31; b < p.B; b += 32) {
+        int start;
+        tokens = min(tokens + (unsigned)max(new_tokens(p, b, start), 0), 1u << 31);
+    }
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) tokens = min(tokens + __shfl_xor_sync(0xffffffffu, tokens, o), 1u << 31);
+    return tokens > (unsigned)p.T;
+}
+
 // Block-wide: the range from the lengths on the device (prefix sums over the
 // sequences, THREADS threads).  False: nothing for this CTA.
 template <int THREADS, int PU, int COST, int LEAST>
@@ -158,32 +171,16 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
             w.ord0 += y;
         }
     }
+    misfit = __any_sync(0xffffffffu, misfit);
     if (lane == 31) {
         s_scan[warp] = w.at0;
-        s_scan[WARPS + warp] = (unsigned)w.ord0;
+        s_scan[WARPS + warp] = (unsigned)w.ord0 | (misfit ? 1u << 31 : 0u);  // (below 2^31 where all starts fit)
     }
-    misfit = __syncthreads_or(misfit);
+    __syncthreads();
     const unsigned wu = lane < WARPS ? s_scan[lane] : 0u, ws = lane < WARPS ? s_scan[WARPS + lane] : 0u;
     const unsigned total = __reduce_add_sync(0xffffffffu, wu);
     w.at0 += __reduce_add_sync(0xffffffffu, lane < warp ? wu : 0u) - w.units;
-    w.ord0 += (int)__reduce_add_sync(0xffffffffu, lane < warp ? ws : 0u) - spans;
-    if (misfit) {
-        // starts that fall may give the same rows to many sequences, and these more units than 32 bits hold: nothing
-        // is begun where they bring more than T tokens together (1e-3 is more than fp32 rounds 2100 terms)
-        float tokens = 0.f;
-        for (int b = w.b_lo; b < w.b_hi; ++b) {
-            int start;
-            if (threadIdx.x % (1u << share) == 0) tokens += (float)max(new_tokens(p, b, start), 0);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
-        __syncthreads();
-        if (lane == 0) s_scan[warp] = __float_as_uint(tokens);
-        __syncthreads();
-        tokens = 0.f;
-        for (int i = 0; i < WARPS; ++i) tokens += __uint_as_float(s_scan[i]);
-        if (tokens > (float)p.T * 1.001f) return false;
-    }
+    w.ord0 += (int)__reduce_add_sync(0xffffffffu, lane < warp ? ws & 0x7fffffffu : 0u) - spans;
     w.per = max((unsigned)LEAST, (total + gridDim.x - 1) / gridDim.x);
     w.lo = min(total, blockIdx.x * w.per);
     w.hi = min(total, w.lo + w.per);
@@ -215,6 +212,8 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     __syncthreads();
     w.first = (int)s_scan[2 * WARPS];
     w.nspans = (int)s_scan[2 * WARPS + 1] - w.first + 1;
+    // (here and not in front of it all: the same code there makes prompts at head_dim 256 1 % slower)
+    if (__any_sync(0xffffffffu, lane < WARPS && s_scan[WARPS + lane] >> 31) && a8_overlap(p)) w.nspans = 0;
     return w.nspans > 0;  // (a range may hold nothing but such a cost)
 }
 
