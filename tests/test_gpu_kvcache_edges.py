@@ -199,3 +199,19 @@ def test_append_rows_far_apart(cache, gap):
     slots[at] = a.slots
     a.slots = slots
     a.check()
+
+
+# ---------------------------------------------------------------------------
+# Nothing at all.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_batch_without_sequences(dtype):
+    a = Attention(38, 4, 2, 64, [(1, 20)], dtype)
+    a.q, a.out = a.q[:0], a.out[:0]
+    a.starts, a.ctx, a.tables = [0], [], np.zeros((0, 4), np.int32)
+    a.call()
+    b = Append(39, 4, 2, 64, [(1, 20)])
+    pool = b.pool.clone()
+    b.call(0, 0)
+    torch.cuda.synchronize()
+    assert int(a.err) == 0 and int(b.err) == 0 and torch.equal(pool, b.pool)

@@ -706,7 +706,7 @@ yk_status attention_e4m3_check(const yk_attention_e4m3_args& a) {
     YK_TRY(kv_pages_check(a.pages, a.layer));
     YK_ARG(a.pages.kind == YK_KV_E4M3, "pages.kind must be YK_KV_E4M3");
     YK_ARG(a.dtype == YK_DTYPE_F32 || a.dtype == YK_DTYPE_BF16, "dtype");
-    YK_ARG(a.T >= 0 && a.B > 0 && a.B <= (1 << 20), "T must not be negative, B in 1..2^20");
+    YK_ARG(a.T >= 0 && a.B >= (a.T > 0 ? 1 : 0) && a.B <= (1 << 20), "T must not be negative, B in 1..2^20 (0 where T is)");
     YK_ARG(a.n_heads > 0 && a.n_heads <= 65536 && a.n_heads % a.pages.n_kv_heads == 0,
            "n_heads must be a positive multiple of n_kv_heads");
     YK_ARG(a.n_heads / a.pages.n_kv_heads <= 1024, "at most 1024 query heads share a KV head");
