@@ -28,8 +28,8 @@
 // and rescales O^T in TMEM).  What lies 2^-28 below a row's largest weight is
 // lost: f16 ends at 2^-25, rounded.
 //
-// Measured, 32 query and 8 KV heads of 128: one token over 131,000 keys 56 us (268
-// MB, 4.8 TB/s: 73 % of a copy's rate); 64 sequences of 2k-8k keys, 5 tokens, 16
+// Measured, 32 query and 8 KV heads of 128: one token over 131,000 keys 57 us (268
+// MB, 4.7 TB/s: 72 % of a copy's rate); 64 sequences of 2k-8k keys, 5 tokens, 16
 // heads of 256, capped, 280 us (73 %); 32 sequences of 512-2048 keys, 6 tokens, 41
 // us (88 MB, 33 %).  Long ranges run at 1800 cycles a tile where the bytes alone
 // need 1400; a tile's fixed cost bounds them (every role is busy for 1100-1500
