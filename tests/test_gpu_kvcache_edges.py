@@ -215,3 +215,40 @@ def test_a_batch_without_sequences(dtype):
     b.call(0, 0)
     torch.cuda.synchronize()
     assert int(a.err) == 0 and int(b.err) == 0 and torch.equal(pool, b.pool)
+
+
+# ---------------------------------------------------------------------------
+# Scores that fp32 holds to whole numbers or worse.
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,max_new", SHAPES)
+@pytest.mark.parametrize("dh", [64, 128, 256])
+@pytest.mark.parametrize("q_std,cap", [(1e6, 0.0), (3e7, 0.0), (1e9, 0.0), (1e14, 0.0), (1e14, 1e30), (1e9, 1e9)])
+def test_huge_scores_give_means_of_values(dtype, max_new, dh, q_std, cap):
+    """A result lies among the values that its query sees; where one score leads by more than the scores' error,
+    spread * (dh + 8) * 2^-23 each and with a cap 2^-20 of themselves (its tanh: the series' next term is 2^-21.5 of the
+    sum at most, the quotient beyond it 2^-22 where it is a quarter), it is that key's value."""
+    lens = [(3, 40), (40, 300), (1, 700)]
+    a = Attention(40, 4, 2, dh, lens, dtype, q_std=q_std)
+    a.call(max_new=max_new, cap=cap)
+    torch.cuda.synchronize()
+    got, half, t = a.out.double().cpu(), torch.finfo(a.out.dtype).eps / 2, 0
+    assert torch.isfinite(got).all() and int(a.err) == 0
+    led = 0
+    for b, (n, c) in enumerate(lens):
+        ids = [int(i) for i in a.tables[b][:(c + 15) // 16]]
+        kv = ref.decode(a.pool[ids, 1].cpu(), a.scales[ids, 1].cpu()).permute(1, 2, 0, 3, 4).reshape(2, 2, -1, dh)
+        for i in range(n):
+            for h in range(4):
+                K, V = kv[0, h // 2, :c - n + i + 1], kv[1, h // 2, :c - n + i + 1]
+                q, y = a.q[t, h].double().cpu(), got[t, h]
+                slack = V.abs().amax(0) * (half + 2.0 ** -11) + V.abs().max() * 2.0 ** -26
+                assert (y >= V.amin(0) - slack).all() and (y <= V.amax(0) + slack).all()
+                x, d = K @ q * dh ** -0.5, float((K.abs() @ q.abs()).max()) * dh ** -0.5 * (dh + 8) * 2.0 ** -23
+                if cap:
+                    x = cap * torch.tanh(x / cap)
+                top = x.topk(min(2, len(x)))
+                if len(x) == 1 or top.values[0] - top.values[1] > 2 * d + (2 * float(x.abs().max()) * 2.0 ** -20 if cap else 0) + 40:
+                    led += 1
+                    assert ((y - V[top.indices[0]]).abs() <= slack).all()
+            t += 1
+    assert led > 0 or cap == 1e9

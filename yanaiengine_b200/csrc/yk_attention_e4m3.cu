@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(A8_THREADS, A8_CTAS) attn8_kernel(const __grid
                     bool over = false;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        over |= fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + 15.f || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + 15.f;
+                        over |= fmaxf(s[nt][0], s[nt][2]) - m[nt][0] > 15.f || fmaxf(s[nt][1], s[nt][3]) - m[nt][1] > 15.f;
                     if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)

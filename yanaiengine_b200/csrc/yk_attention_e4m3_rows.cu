@@ -91,6 +91,25 @@ static __device__ __noinline__ void finish_scores(uint32_t s_at, const int* info
     tmem_wait_st();
 }
 
+// Scores -> what the weights are 2^ of, in TMEM: rounded as the row's largest was when its reference was taken from it.
+// (Where fp32 holds scores to whole numbers or worse, a product that is not rounded before the reference is taken off may
+// lie above the largest by more than f16 has room for.)
+static __device__ __noinline__ void settle_scores(uint32_t s_at, const int* info, float rf, bool raw, float now) {
+#pragma unroll 1
+    for (int b = 0; b < TCA_PAGES; ++b) {
+        uint32_t x[16];
+        const int w = info[b];
+        tmem_ld<16>(s_at + 16 * b, x);
+        const float f = raw ? score_factor(w, rf) : 1.f, ev = (float)(w >= 0 ? (w >> 8) - 128 : 0);
+        tmem_wait_ld();
+        settle(x);
+#pragma unroll
+        for (int z = 0; z < 16; ++z) x[z] = __float_as_uint(fmaf(__uint_as_float(x[z]), f, ev) - now);
+        tmem_st<16>(s_at + 16 * b, x);
+    }
+    tmem_wait_st();
+}
+
 template <int DH>
 __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ Attn8Params p) {
     using C = TcrCfg<DH>;
@@ -240,13 +259,21 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                     // would pass 2^15
                     if (t > 0) pair_wait(group ^ 1, quad);
                     float now = i == 0 ? A8_LOWEST : s_m[row];
-                    const bool over = top > now + 15.f, moves = __any_sync(0xffffffffu, over) && i > 0;
+                    const bool over = top - now > 15.f, moves = __any_sync(0xffffffffu, over) && i > 0;
                     const float was = now;
                     if (over) now = top - 3.f;
                     s_m[row] = now;
                     if (i + 1 < n || si + 1 < nseg || seg0 + A8_SEGS < work.nspans) pair_tell(group, quad);  // (not after the last tile)
                     l *= ex2(m - now);
                     m = now;
+                    // (one reference of the warp's 32 from 2^22 on: all of them the long way)
+                    const bool far = __any_sync(0xffffffffu, fabsf(now) >= 4194304.f && now != A8_LOWEST);
+                    if (far) {
+                        tmem_wait_ld();
+                        settle_scores(s_at, info, rf, raw, now);
+                        tmem_ld<16>(s_at, x[0]);
+                        raw = false;
+                    }
                     wait(p_empty + 8 * group, (use & 1) ^ 1);
                     tc_fence_after();
 #pragma unroll 1
@@ -259,7 +286,7 @@ __global__ void __launch_bounds__(TCR_THREADS, 1) attn8_rows_kernel(const __grid
                             settle(y);
                             if (u == 0 || b + 2 < TCA_PAGES) tmem_ld<16>(s_at + (uint32_t)(16 * (b + u + 1)), x[u ^ 1]);
                             const int word = u ? w.y : w.x, ev = word >= 0 ? (word >> 8) - 128 : 0;
-                            const float f = raw ? score_factor(word, rf) : 1.f, c = (float)ev - now;
+                            const float f = raw ? score_factor(word, rf) : 1.f, c = far ? 0.f : (float)ev - now;
                             const float2 ff = make_float2(f, f), cc = make_float2(c, c);
                             float2 sum = make_float2(0.f, 0.f);
                             uint32_t h[8];

@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                         uint32_t x[BATCH], y[C::JOINED ? 1 : BATCH];
                         tmem_ld<BATCH>(at + (uint32_t)b0, x);
                         if constexpr (!C::JOINED) tmem_ld<BATCH>(at + (uint32_t)(R + b0), y);
-                        float4 f[BATCH / 4], m[BATCH / 4];  // (these come while the scores do)
+                        // (these come while the scores do; a score is rounded before its reference, which was taken from a rounded
+                        // one, is taken off: where fp32 holds scores to whole numbers the difference counts)
+                        float4 f[BATCH / 4], m[BATCH / 4];
 #pragma unroll
                         for (int n = 0; n < BATCH / 4; ++n) {
                             f[n] = *reinterpret_cast<const float4*>(rf + b0 + 4 * n);
@@ -255,8 +257,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
                             if constexpr (!C::JOINED)
                                 s = fma2(make_float2(__uint_as_float(y[n]), __uint_as_float(y[n + 1])), make_float2(0.0625f, 0.0625f), s);
                             const float2 r = n & 2 ? make_float2(ff.z, ff.w) : make_float2(ff.x, ff.y);
-                            const float2 c = fma2(n & 2 ? make_float2(mm.z, mm.w) : make_float2(mm.x, mm.y), now, first);
-                            d[(b0 + n) / 2] = fma2(mul2(s, fk2), r, c);
+                            d[(b0 + n) / 2] = fma2(n & 2 ? make_float2(mm.z, mm.w) : make_float2(mm.x, mm.y), now, fma2(mul2(s, fk2), r, first));
                         }
                     }
                     tc_fence_before();
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(TCA_THREADS, 1) attn8_tc_kernel(const __grid_c
 #pragma unroll
                         for (int n = 0; n < RH; n += 2) {
                             const float2 m = *reinterpret_cast<const float2*>(s_neg + r0 + n);
-                            d[n / 2] = add2(make_float2(cap_score(p, d[n / 2].x), cap_score(p, d[n / 2].y)), add2(shift, m));
+                            d[n / 2] = add2(add2(make_float2(cap_score(p, d[n / 2].x), cap_score(p, d[n / 2].y)), shift), m);
                         }
                     }
                     if (!plain) {
