@@ -212,7 +212,8 @@ __device__ __forceinline__ bool a8_plan(const Attn8Params& p, int R, int rep, un
     __syncthreads();
     w.first = (int)s_scan[2 * WARPS];
     w.nspans = (int)s_scan[2 * WARPS + 1] - w.first + 1;
-    // (here and not in front of it all: the same code there makes prompts at head_dim 256 1 % slower)
+    // where some starts do not fit (looked for here and not in front of it all: the same code there makes prompts at
+    // head_dim 256 1 % slower)
     if (__any_sync(0xffffffffu, lane < WARPS && s_scan[WARPS + lane] >> 31) && a8_overlap(p)) w.nspans = 0;
     return w.nspans > 0;  // (a range may hold nothing but such a cost)
 }
